@@ -802,6 +802,79 @@ int swr_block_select_fwd(const float* V, int64_t ldv, const void* domain, int do
 int swr_block_select_bwd(const float* dout, int64_t ldo, const void* domain, int dom_dtype, int D, int H, int64_t M,
                          float* dV, int64_t ldv, void* stream);
 
+/* ------------------------------------------------------------ sequence attention ----
+ * Self-attention over behaviour histories: packed sequences, grouped heads, a learned position bias by buckets (no reference
+ * counterpart: the reference pools a history by sum / mean / concat, basic/layers.py:174-228).
+ *   s_ij = scale q_i . k_j + bias[h, buckets[entry(i + lk - lq - j)]]      i < lq, j < lk of one sequence, h = query head
+ *   out_i = sum_j softmax_j(s_ij) v_j over the allowed j: key_mask[j] != 0 and, causal, j <= i + lk - lq
+ * A row with no allowed key is zeros, and so are its gradients.  Query head h reads key head h / (Hq / Hk).
+ * Sequence b: query rows cu_q[b] .. cu_q[b + 1], key rows cu_k[b] .. cu_k[b + 1] (prefix sums, int32, B + 1 entries); q_len / k_len
+ * (nullable, [B]) = how many of them are in use.  Rows that are in no sequence or not in use come out as zeros.  A prefix or length
+ * outside its range is clamped and raises SWR_FLAG_INDEX_OOR, as does a bucket outside [0, n_buckets).
+ * entry(d): causal min(d, n_dist - 1); else n_dist = 2 R + 1 and clamp(d, -R, R) + R.  n_dist = 0: no bias.
+ * q, k, v, dout: element strides row / head, unit stride inside a head; out, dq, dk, dv: contiguous [rows, heads, D], 16-byte aligned.
+ * dtype SWR_F32 (products of three bf16 terms per value, fp32 accuracy) or SWR_BF16; bias, dbias, lse are fp32.
+ * max_q / max_k: longest sequence -- they choose the launch and its tiling (right for any value, other values round differently).
+ * Deterministic: fixed summation orders, no atomics on results. */
+#define SWR_SEQ_MAX_DIM 128
+#define SWR_SEQ_MAX_DIST 4097
+#define SWR_SEQ_MAX_BUCKETS 256
+#define SWR_SEQ_MAX_TABLE 8192          /* n_dist * (Hq / Hk): the bias rows of a group are held in LDS */
+typedef struct {
+    int64_t Tq, Tk;                    /* rows of q / out and of k / v */
+    int32_t B, Hq, Hk, D;
+    int32_t dtype, causal, max_q, max_k;
+    float scale;
+    int32_t n_dist, n_buckets, pad;
+    const void* q; int64_t q_row, q_head;
+    const void* k; int64_t k_row, k_head;
+    const void* v; int64_t v_row, v_head;
+    void* out;
+    float* lse;                        /* [Hq, Tq] log2 of the softmax sums, +inf for an empty row; NULL in a forward without a backward */
+    const int32_t* cu_q; const int32_t* cu_k; const int32_t* q_len; const int32_t* k_len;
+    const uint8_t* key_mask;           /* [Tk], nullable */
+    const float* bias;                 /* [Hq, n_buckets] */
+    const int32_t* buckets;            /* [n_dist] */
+    const void* dout; int64_t do_row, do_head;
+    void* dq; void* dk; void* dv;
+    float* dbias;                      /* [Hq, n_buckets], nullable, overwritten */
+    uint32_t* err_flag;                /* nullable */
+} swr_seq_attention_args;
+size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_args* a);
+int swr_seq_attention_fwd(const swr_seq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
+size_t swr_seq_attention_bwd_workspace_bytes(const swr_seq_attention_args* a);
+int swr_seq_attention_bwd(const swr_seq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------ norms around a block ----
+ * The root-mean-square norms behind one block and before the next, fused with the block's gate and residual (no reference counterpart;
+ * beside swr_layernorm_* and swr_mul_sigmoid_*):
+ *   t = y rms(y) w_post    (w_post NULL: t = y)         rms(a) = 1 / sqrt(mean of a^2 over the row + eps)
+ *   z = x + scale sigmoid(gate) t                       (gate NULL: without the sigmoid; y NULL: z = x, not written)
+ *   u = z rms(z) w_pre     (w_pre NULL: no u)           z enters unrounded
+ * Rows of N <= SWR_NORM_GATE_MAX_WIDTH elements of `dtype` (SWR_F32 / SWR_BF16); x, y, gate, dz, du have leading dimensions, z, u, dx,
+ * dy, dgate are contiguous; weights, their gradients and ry / rz ([M], kept for the backward; nullable in a forward without one) fp32.
+ * Backward: dz and du nullable (a missing one counts as zeros), dx, dy, dgate overwritten, dw_post / dw_pre nullable, overwritten,
+ * fixed-order column sums (workspace needed when one of them is asked for). */
+#define SWR_NORM_GATE_MAX_WIDTH 8192
+typedef struct {
+    int64_t M;
+    int32_t N, dtype;
+    float eps, scale;
+    const void* x; int64_t ldx;
+    const void* y; int64_t ldy;
+    const void* gate; int64_t ldg;
+    const float* w_post; const float* w_pre;
+    void* z; void* u;
+    float* ry; float* rz;
+    const void* dz; int64_t lddz;
+    const void* du; int64_t lddu;
+    void* dx; void* dy; void* dgate;
+    float* dw_post; float* dw_pre;
+} swr_norm_gate_args;
+int swr_norm_gate_fwd(const swr_norm_gate_args* a, void* stream);
+size_t swr_norm_gate_bwd_workspace_bytes(int64_t M, int N);
+int swr_norm_gate_bwd(const swr_norm_gate_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ input columns ----
  * Row permutation of a columnar, device-resident dataset (replaces DataLoader(shuffle=True) over
  * TorchDataset, whose __getitem__ builds one python dict per ROW, utils/data.py:11-22,55): for every column c,

@@ -1,0 +1,314 @@
+// Device pieces shared by the sequence-attention kernels (seq_attention_fwd.hip, seq_attention_bwd.hip).
+//
+// Every product runs on v_mfma_f32_32x32x16_bf16.  NP = bf16 planes per value: 1 for bf16 tensors, 3 for fp32 ones (x = h + m + l,
+// split3.h; six plane products of order <= 2^-16 each, what is dropped is below 2^-24 of the operands' product).  DP = the head
+// width padded to 32, 64 or 128 (columns beyond D are zeros in LDS).
+//
+// A 32 x 32 result tile: lane l holds column l & 31 and the rows 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0 .. 15.  The kernels put the
+// rows of softmax statistics on COLUMNS (one lane pair per row, no broadcast) and reuse a result tile as the right operand of the
+// next product without moving it between lanes: the 16 contraction indices of a step are then {4 hi + 0..3, 8 + 4 hi + 0..3} per half
+// wave hi, and the left operand is read from LDS in the same order (lds_tr, ds_read_b64_tr_b16: 4 rows of one column per lane).
+//
+// LDS tile: [rows][DP] bf16 per plane, 16-byte pieces XOR-swizzled by row so that both readers are free of bank conflicts: the row
+// reader (16 consecutive rows, one piece each) and the transposing one (4 consecutive rows x 64 bytes per half wave).
+#pragma once
+#include "common.h"
+#include "split3.h"
+#include "vec8.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) char* sa_lds;
+typedef __attribute__((address_space(3))) bf16x4* sa_lds_tr;
+typedef __attribute__((address_space(3))) bf16x8* sa_lds_v;
+
+#define SA_LOG2E 1.4426950408889634f
+
+struct SaK {
+    int64_t Tq, Tk;
+    int B, Hq, Hk, G, D, causal;
+    float c;                               // scale * log2(e)
+    float scale;
+    int n_dist, n_buckets, reach;          // reach: largest |distance| with an entry of its own
+    int vq, vk, vv, vo, vdo;               // elements per load of q, k, v, out, dout rows: 8, 4 or 1
+    bool fast;                             // all of them 8, row strides below 2^23 elements (64 rows within 32-bit byte offsets)
+    const void *q, *k, *v; int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    void* out; float* lse;
+    const int32_t *cu_q, *cu_k, *q_len, *k_len;
+    const uint8_t* key_mask;
+    const float* bias; const int32_t* buckets;
+    const void* dout; int64_t do_row, do_head;
+    void *dq, *dk, *dv; float* dbias;
+    uint32_t* err_flag;
+    // launch geometry
+    int tiles, per_unit, units;            // column tiles per sequence, workgroups per (sequence, key head), B * Hk
+    int pack;                              // query heads side by side in the columns (1 or G)
+    int splits;                            // workgroups per key range
+    float* part;                           // forward, splits > 1: [splits][Hq][Tq] (max, sum), then [splits][Hq][Tq][D]
+    float* delta;                          // backward: [Hq][Tq]
+    float* bias_part; int bias_slots;      // backward: [Hq][n_buckets][bias_slots]
+};
+
+// one sequence: first rows, rows present (the cu arrays' span), rows in use (q_len / k_len)
+struct SaSeq {
+    int64_t q0, k0;
+    int q_span, k_span, lq, lk, shift;     // shift = lk - lq: query i stands at key position i + shift
+};
+__device__ __forceinline__ int64_t sa_clamp(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }
+__device__ __forceinline__ SaSeq sa_seq(const SaK& a, int b) {
+    SaSeq s;
+    const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+    s.q0 = sa_clamp(q0, 0, a.Tq);
+    s.k0 = sa_clamp(k0, 0, a.Tk);
+    s.q_span = static_cast<int>(sa_clamp(q1, s.q0, a.Tq) - s.q0);
+    s.k_span = static_cast<int>(sa_clamp(k1, s.k0, a.Tk) - s.k0);
+    int lq = s.q_span, lk = s.k_span;
+    bool bad = q0 < 0 || q1 < q0 || q1 > a.Tq || k0 < 0 || k1 < k0 || k1 > a.Tk;
+    if (a.q_len) { const int n = a.q_len[b]; bad |= n < 0 || n > lq; lq = max(0, min(n, lq)); }
+    if (a.k_len) { const int n = a.k_len[b]; bad |= n < 0 || n > lk; lk = max(0, min(n, lk)); }
+    s.lq = lq; s.lk = lk; s.shift = lk - lq;
+    if (bad && a.err_flag && threadIdx.x == 0) atomicOr(a.err_flag, SWR_FLAG_INDEX_OOR);
+    return s;
+}
+
+template <int NP> struct SaT { typedef uint16_t type; };
+template <> struct SaT<3> { typedef float type; };
+template <int NP> using SaRaw = Raw8<typename SaT<NP>::type>;
+// -> the planes of 8 values
+__device__ __forceinline__ void sa_planes(const Raw8<uint16_t>& r, bf16x8 (&o)[1]) { o[0] = __builtin_bit_cast(bf16x8, r.v); }
+__device__ __forceinline__ void sa_split8(const float* f, bf16x8 (&o)[3]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) SPLIT3_PAIR(f[j], f[j + 1], o[0], o[1], o[2], j);
+}
+__device__ __forceinline__ void sa_planes(const Raw8<float>& r, bf16x8 (&o)[3]) {
+    float f[8];
+    floats8(r, f);
+    sa_split8(f, o);
+}
+// 8 fp32 values (probabilities, score gradients) as a right operand: rounded to bf16 once for bf16 tensors (2^-9 relative, the size
+// of the rounding of the outputs themselves), split exactly for fp32 ones
+__device__ __forceinline__ void sa_planes_f(const float* f, bf16x8 (&o)[3]) { sa_split8(f, o); }
+__device__ __forceinline__ void sa_planes_f(const float* f, bf16x8 (&o)[1]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) CVT_PAIR(f[j], f[j + 1], o[0], j);
+}
+
+__device__ __forceinline__ f32x16 sa_mma(const bf16x8 (&a)[1], const bf16x8 (&b)[1], f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 sa_mma(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], c, 0, 0, 0);     // smallest terms first
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 sa_zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// ---- LDS tile
+template <int DP>
+__device__ __forceinline__ int sa_swz(int row) {
+    if (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    if (DP == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    return (row >> 2) & 3;
+}
+template <int DP>
+__device__ __forceinline__ int sa_off(int row, int chunk) { return row * (DP * 2) + ((chunk ^ sa_swz<DP>(row)) << 4); }
+
+// R rows of a [*, DP] operand moved by NT threads: global -> registers (load), registers -> LDS planes (store).
+// FAST: 16-byte rows and D % 8 == 0 -- every lane loads from a valid address (the last row, the first columns) without a branch and
+// what it should not have read becomes zeros on the way to LDS.  Otherwise 4 or 1 elements at a time under their conditions.
+template <int NP, int DP, int R, int NT, bool FAST>
+struct SaStage {
+    static constexpr int CPR = DP / 8, N = R * CPR / NT, STEP = NT / CPR;
+    static_assert(R * CPR % NT == 0 && NT % CPR == 0, "whole chunks per thread");
+    static constexpr int PLANE = R * DP * 2, BYTES = NP * PLANE;
+    typedef typename SaT<NP>::type T;
+    SaRaw<NP> r[N];
+    uint32_t keep;                         // bit i: r[i] counts (rows in use, not masked)
+    // rows first .. first + R - 1 of a sequence whose row 0 is `row0`; rows >= limit (limit > first) or masked read as zeros
+    __device__ __forceinline__ void load(const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D, int vw,
+                                         const uint8_t* mask) {
+        const int chunk = threadIdx.x % CPR, row = threadIdx.x / CPR;
+        const T* p = static_cast<const T*>(base) + (row0 + first) * stride + head_off;
+        keep = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int rr = row + i * STEP;
+            bool ok = first + rr < limit;
+            const int rc = min(rr, limit - 1 - first);
+            if (FAST) {
+                r[i] = load8(p + static_cast<uint32_t>(rc) * static_cast<uint32_t>(stride) + (chunk * 8 < D ? chunk * 8 : 0), 8, 8);
+                ok = ok && chunk * 8 < D;
+            }
+            if (mask) ok = ok && mask[row0 + first + rc] != 0;
+            if (!FAST) r[i] = load8(p + rc * stride + chunk * 8, ok ? D - chunk * 8 : 0, vw);
+            keep |= static_cast<uint32_t>(ok) << i;
+        }
+    }
+    __device__ __forceinline__ void store(sa_lds dst) const {
+        const int chunk = threadIdx.x % CPR, row = threadIdx.x / CPR;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            SaRaw<NP> x = r[i];
+            if (FAST && !((keep >> i) & 1)) x = zero8(x);
+            bf16x8 p[NP];
+            sa_planes(x, p);
+            const int off = sa_off<DP>(row + i * STEP, chunk);
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) *reinterpret_cast<sa_lds_v>(dst + pl * PLANE + off) = p[pl];
+        }
+    }
+};
+
+// The same by LDS-DMA (bf16, FAST): 16-byte copies from HBM into the tile, no registers and no VALU in between.  The swizzle is in the
+// source address (LDS places are lane-linear); rows and columns that do not count copy a zero piece.  Inline asm because the compiler
+// would wait for every copy in flight in front of each LDS read; the kernels wait themselves (sa_dma_wait) before the barrier that
+// hands a tile over.
+static __device__ __attribute__((aligned(16))) uint32_t sa_zero_piece[4];
+__device__ __forceinline__ void sa_dma16(uint32_t lds_addr, const void* src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void sa_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int DP, int R, int NT>
+struct SaDma {
+    static constexpr int CPR = DP / 8, N = R * CPR / NT, STEP = NT / CPR;
+    static_assert(R * CPR % NT == 0 && NT % CPR == 0, "whole chunks per thread");
+    static __device__ __forceinline__ void copy(sa_lds dst, const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D,
+                                                const uint8_t* mask) {
+        const int slot = threadIdx.x % CPR, row = threadIdx.x / CPR;
+        const uint16_t* p = static_cast<const uint16_t*>(base) + (row0 + first) * stride + head_off;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)) + (threadIdx.x & ~63u) * 16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int rr = row + i * STEP, col = (slot ^ sa_swz<DP>(rr)) * 8;
+            bool ok = first + rr < limit && col < D;
+            if (mask) ok = ok && mask[row0 + first + rr] != 0;
+            sa_dma16(at + i * NT * 16, ok ? static_cast<const void*>(p + static_cast<uint32_t>(rr) * static_cast<uint32_t>(stride) + col)
+                                          : static_cast<const void*>(sa_zero_piece));
+        }
+    }
+};
+
+// left operand of a product over the columns: row (lane & 31) of block rb, columns 16 s + 8 hi .. + 7
+template <int NP, int DP, int R>
+__device__ __forceinline__ void sa_rows(sa_lds tile, int rb, int s, int lane, bf16x8 (&o)[NP]) {
+    const int off = sa_off<DP>(rb * 32 + (lane & 31), 2 * s + (lane >> 5));
+#pragma unroll
+    for (int pl = 0; pl < NP; ++pl) o[pl] = *reinterpret_cast<sa_lds_v>(tile + pl * (R * DP * 2) + off);
+}
+// left operand of a product over the rows: column 32 db + (lane & 31), rows 16 ks + {4 hi + 0..3, 8 + 4 hi + 0..3}
+template <int NP, int DP, int R>
+__device__ __forceinline__ void sa_cols(sa_lds tile, int ks, int db, int lane, bf16x8 (&o)[NP]) {
+    const int row = 16 * ks + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int chunk = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), half = (lane & 1) * 8;
+    const int o0 = sa_off<DP>(row, chunk) + half, o1 = sa_off<DP>(row + 8, chunk) + half;
+#pragma unroll
+    for (int pl = 0; pl < NP; ++pl) {
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(tile + pl * (R * DP * 2) + o0));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(tile + pl * (R * DP * 2) + o1));
+        o[pl] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+// right operand held in registers: row `off` (elements) of a matrix, columns 16 s + 8 hi .. + 7 (zeros beyond D or where !ok)
+// (FAST: `off` has to be a valid row where !ok, too)
+template <int NP, bool FAST>
+__device__ __forceinline__ SaRaw<NP> sa_row8(const void* base, int64_t off, int col, bool ok, int D, int vw) {
+    const typename SaT<NP>::type* p = static_cast<const typename SaT<NP>::type*>(base) + off;
+    if (!FAST) return load8(p + col, ok ? D - col : 0, vw);
+    const SaRaw<NP> x = load8(p + (col < D ? col : 0), 8, 8);
+    return ok && col < D ? x : zero8(x);
+}
+template <int NP, int DP, bool FAST>
+__device__ __forceinline__ void sa_row_frags(const void* base, int64_t off, bool ok, int D, int vw, int lane, bf16x8 (&o)[DP / 16][NP]) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) sa_planes(sa_row8<NP, FAST>(base, off, 16 * s + 8 * (lane >> 5), ok, D, vw), o[s]);
+}
+
+// ... kept as loaded and split at every use where the planes of two operands do not fit the registers (fp32, D > 64: 192 of them)
+template <int NP, int DP, bool FAST, bool SPLIT_LATE>
+struct SaRows {
+    bf16x8 p[DP / 16][NP];
+    __device__ __forceinline__ void load(const void* base, int64_t off, bool ok, int D, int vw, int lane) {
+        sa_row_frags<NP, DP, FAST>(base, off, ok, D, vw, lane, p);
+    }
+    __device__ __forceinline__ void get(int s, bf16x8 (&o)[NP]) const {
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) o[pl] = p[s][pl];
+    }
+};
+template <int NP, int DP, bool FAST>
+struct SaRows<NP, DP, FAST, true> {
+    SaRaw<NP> r[DP / 16];
+    __device__ __forceinline__ void load(const void* base, int64_t off, bool ok, int D, int vw, int lane) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) r[s] = sa_row8<NP, FAST>(base, off, 16 * s + 8 * (lane >> 5), ok, D, vw);
+    }
+    __device__ __forceinline__ void get(int s, bf16x8 (&o)[NP]) const {
+        float f[8];
+        floats8(r[s], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(f[j]));       // (the split stays in the loop: hoisted, its planes spill)
+        sa_split8(f, o);
+    }
+};
+
+// 4 consecutive result columns d .. d + 3 of a row at `p` (row of D elements)
+template <int NP>
+__device__ __forceinline__ void sa_store4(void* base, int64_t row_off, int d, int D, const float* x) {
+    if (d >= D) return;
+    if (NP == 3) {
+        float* p = static_cast<float*>(base) + row_off + d;
+        if ((D & 3) == 0) {
+            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < D) p[j] = x[j];
+        }
+    } else {
+        uint16_t* p = static_cast<uint16_t*>(base) + row_off + d;
+        bf16x4 v;
+        CVT_PAIR(x[0], x[1], v, 0);
+        CVT_PAIR(x[2], x[3], v, 2);
+        const uint2 w = __builtin_bit_cast(uint2, v);
+        if ((D & 3) == 0) {
+            *reinterpret_cast<uint2*>(p) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < D) p[j] = static_cast<uint16_t>((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
+        }
+    }
+}
+
+// ---- workgroup -> (unit = sequence and key head, work item inside it).  Consecutive workgroups go to the 8 XCDs in turn: all
+// workgroups of a unit stay on one XCD, whose L2 then holds the unit's keys and values once.
+__device__ __forceinline__ int sa_unit(int id, int per_unit, int& within) {
+    const int slot = id >> 3;
+    within = slot % per_unit;
+    return (slot / per_unit) * 8 + (id & 7);
+}
+
+// entry of the distance table, clamped to its reach (causal: distances 0 .. reach, else -reach .. reach)
+__device__ __forceinline__ int sa_entry(int dist, int reach, int causal) {
+    return causal ? max(0, min(dist, reach)) : max(-reach, min(dist, reach)) + reach;
+}
+// bias in the exponent's base-2 unit; a finite value stays finite (a bias of the type's lowest value masks relative to the row's
+// other scores, it does not empty the row)
+__device__ __forceinline__ float sa_bias2(float b) {
+    const float x = b * SA_LOG2E;
+    return (__builtin_isinf(x) && !__builtin_isinf(b)) ? copysignf(3.402823466e38f, x) : x;
+}
+// rows outside every sequence (before the first, behind the last) are zeros in every output
+__device__ __forceinline__ void sa_zero_rows(void* base, int elem, int64_t r0, int64_t r1, int64_t row_elems, int nthreads, int part, int parts) {
+    char* p = static_cast<char*>(base);
+    const int64_t n0 = r0 * row_elems * elem, n1 = r1 * row_elems * elem;
+    for (int64_t i = n0 + 2 * (static_cast<int64_t>(part) * nthreads + threadIdx.x); i < n1; i += 2ll * nthreads * parts)
+        *reinterpret_cast<uint16_t*>(p + i) = 0;
+}

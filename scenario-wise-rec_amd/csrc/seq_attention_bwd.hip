@@ -1,0 +1,483 @@
+// Attention over packed sequences, backward (seq_attention_fwd.hip has the forward and its definitions).
+//
+//   p_ij = 2^(x_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,   dbias[h, t] = sum of ds over bucket t
+//
+// Two passes that recompute the scores, so that every sum has one owner and a fixed order (no atomics): a workgroup of query columns
+// walks the keys and holds dq (it also makes delta and the bias gradient), a workgroup of key columns walks the queries of all heads
+// of its group and holds dk and dv.  7 products instead of 5, against the fp32 read-modify-write of dq for every key tile.
+//
+// Bias gradient: a 32 x 32 block of ds has 63 distances.  Its wave writes it to LDS so that a distance becomes a row-wise constant
+// column (row k at offset -k), lane t adds up distance t and owns that entry of the wave's per-distance sums.  Blocks wholly beyond
+// the table's reach add their sum to one register.
+#include <algorithm>
+
+#include "seq_attention.h"
+
+int sa_check(const swr_seq_attention_args* p, bool backward);
+SaK sa_args(const swr_seq_attention_args* p);
+int sa_waves(int64_t columns, const SaK& a, bool fp32);
+unsigned sa_grid(SaK& a);
+
+// waves per SIMD the registers are bounded for (512 / waves each)
+#define SA_WAVES_DQ(NP, DP) ((NP) * (DP) >= 128 ? 1 : 2)
+#define SA_WAVES_DKV(NP, DP) ((NP) * (DP) >= 128 ? 1 : 2)
+#define SA_SKEW 2048                           // floats of a wave's skewed 32 x 32 block (32 rows of 64)
+
+// dq: DMA and buffers as in the forward; 32 keys a step at DP = 128, so that two workgroups fit a CU's LDS beside the skew blocks
+template <int NP, int DP, int NW, bool FAST>
+struct SaDq {
+    static constexpr bool DMA = FAST && NP == 1;
+    static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
+    static constexpr int TILE = NP * KT * DP * 2;
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.n_dist + (a.bias_part ? NW * (SA_SKEW + a.n_dist) : 0)) * 4; }
+};
+template <int NP, int DP, int NW, bool FAST>
+struct SaDkv {
+    static constexpr bool DMA = FAST && NP == 1, LATE = NP * DP >= 384;       // LATE: splits at use, nothing staged ahead (registers)
+    static constexpr int RT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
+    static constexpr int TILE = NP * RT * DP * 2;
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + 2 * RT * 4) + a.G * a.n_dist * 4; }
+};
+
+__device__ __forceinline__ void sa_bias_rows(const SaK& a, int h, int heads, float* bt, int nthreads) {
+    for (int i = threadIdx.x; i < heads * a.n_dist; i += nthreads)
+        bt[i] = sa_bias2(a.bias[static_cast<int64_t>(h + i / a.n_dist) * a.n_buckets + max(0, min(a.buckets[i % a.n_dist], a.n_buckets - 1))]);
+}
+
+template <int NP, int DP, int NW, bool FAST>
+__global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq_kernel(const SaK a) {
+    typedef SaDq<NP, DP, NW, FAST> Cfg;
+    constexpr int KT = Cfg::KT, KB = KT / 32, NT = NW * 64, QT = NW * 32, TILE = Cfg::TILE;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    uint8_t* km0 = reinterpret_cast<uint8_t*>(smem) + Cfg::NBUF * 2 * TILE;
+    float* bt = reinterpret_cast<float*>(km0 + Cfg::NBUF * KT);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    float* skew = bt + a.n_dist + wave * SA_SKEW;
+    float* acc = bt + a.n_dist + NW * SA_SKEW + wave * a.n_dist;
+
+    int within;
+    const int unit = sa_unit(blockIdx.x, a.per_unit, within);
+    if (unit > a.units) return;
+    if (unit == a.units) {                     // rows of no sequence
+        const int64_t end0 = sa_clamp(a.cu_q[0], 0, a.Tq), beg1 = sa_clamp(a.cu_q[a.B], end0, a.Tq), row = static_cast<int64_t>(a.Hq) * a.D;
+        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, 0, end0, row, NT, within, a.per_unit);
+        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, beg1, a.Tq, row, NT, within, a.per_unit);
+        return;
+    }
+    const int b = unit / a.Hk, hk = unit % a.Hk, g = within % a.G, h = hk * a.G + g, tile0 = a.tiles - 1 - within / a.G;
+    const SaSeq sq = sa_seq(a, b);
+    sa_bias_rows(a, h, 1, bt, NT);
+    if (a.bias_part) {
+        for (int i = lane; i < SA_SKEW; i += 64) skew[i] = 0.f;
+        for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
+    }
+    float beyond_hi = 0.f, beyond_lo = 0.f;    // ds at distances >= reach / <= -reach (this lane's share)
+
+    for (int64_t tile = tile0; tile * QT < sq.q_span; tile += a.tiles) {
+        const int first = static_cast<int>(tile * QT), wfirst = first + wave * 32, tok = wfirst + (lane & 31);
+        const bool exists = tok < sq.q_span, live = tok < sq.lq;
+        const int qpos = tok + sq.shift, wlast = min(wfirst + 31, sq.lq - 1), blast = min(first + QT - 1, sq.lq - 1);
+        int kend = a.causal ? min(sq.lk, blast + sq.shift + 1) : sq.lk;
+        if (first >= sq.lq || kend < 0) kend = 0;
+        const int ntile = (kend + KT - 1) / KT;
+
+        const int64_t row = sq.q0 + (exists ? tok : 0), at = static_cast<int64_t>(h) * a.Tq + row;
+        bf16x8 Q[DP / 16][NP], dO[DP / 16][NP];
+        sa_row_frags<NP, DP, FAST>(a.q, row * a.q_row + static_cast<int64_t>(h) * a.q_head, live, a.D, a.vq, lane, Q);
+        float delta = 0.f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int col = 16 * s + 8 * hi;
+            const SaRaw<NP> x = sa_row8<NP, FAST>(a.dout, row * a.do_row + static_cast<int64_t>(h) * a.do_head, col, live, a.D, a.vdo);
+            const SaRaw<NP> y = sa_row8<NP, FAST>(a.out, (row * a.Hq + h) * a.D, col, live, a.D, a.vo);
+            float fx[8], fy[8];
+            floats8(x, fx);
+            floats8(y, fy);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
+            sa_planes(x, dO[s]);
+        }
+        delta += __shfl_xor(delta, 32);
+        const float lse = live ? a.lse[at] : INFINITY;
+        if (exists && hi == 0) a.delta[at] = delta;
+        f32x16 dQ[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) dQ[db] = sa_zero16();
+
+        SaStage<NP, DP, KT, NT, FAST> sk, sv;
+        uint8_t mk = 1;
+        auto fetch = [&](int t, int buf) {
+            if (Cfg::DMA) {
+                const sa_lds to = (sa_lds)smem + buf * 2 * TILE;
+                SaDma<DP, KT, NT>::copy(to, a.k, sq.k0, t * KT, sq.lk, a.k_row, hk * a.k_head, a.D, a.key_mask);
+                SaDma<DP, KT, NT>::copy(to + TILE, a.v, sq.k0, t * KT, sq.lk, a.v_row, hk * a.v_head, a.D, a.key_mask);
+            } else {
+                sk.load(a.k, sq.k0, t * KT, sq.lk, a.k_row, hk * a.k_head, a.D, a.vk, a.key_mask);
+                sv.load(a.v, sq.k0, t * KT, sq.lk, a.v_row, hk * a.v_head, a.D, a.vv, a.key_mask);
+            }
+            if (a.key_mask && threadIdx.x < KT) {
+                const int key = t * KT + threadIdx.x;
+                mk = key < sq.lk ? a.key_mask[sq.k0 + key] : 0;
+            }
+        };
+        if (ntile > 0) {
+            __syncthreads();
+            fetch(0, 0);
+        }
+        for (int t = 0; t < ntile; ++t) {
+            const int buf = Cfg::DMA ? t & 1 : 0;
+            const sa_lds kt = (sa_lds)smem + buf * 2 * TILE, vt = kt + TILE;
+            const uint8_t* km = km0 + buf * KT;
+            if (Cfg::DMA) {
+                if (a.key_mask && threadIdx.x < KT) km0[buf * KT + threadIdx.x] = mk;
+                sa_dma_wait();
+                __syncthreads();
+            } else {
+                if (t > 0) __syncthreads();
+                sk.store(kt);
+                sv.store(vt);
+                if (a.key_mask && threadIdx.x < KT) km0[threadIdx.x] = mk;
+                __syncthreads();
+            }
+            if (t + 1 < ntile) fetch(t + 1, buf ^ 1);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int k0 = t * KT + kb * 32;
+                if (wfirst > wlast || k0 >= sq.lk || (a.causal && k0 > wlast + sq.shift)) continue;      // (whole waves)
+                f32x16 S = sa_zero16(), dP = sa_zero16();
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                    bf16x8 A[NP];
+                    sa_rows<NP, DP, KT>(kt, kb, s, lane, A);
+                    S = sa_mma(A, Q[s], S);
+                    sa_rows<NP, DP, KT>(vt, kb, s, lane, A);
+                    dP = sa_mma(A, dO[s], dP);
+                }
+                const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
+                const bool apart = near_d >= a.reach || far_d <= -a.reach;                               // one bias for the whole block
+                const bool edge = k0 + 32 > sq.lk || (a.causal && near_d < 0) || a.key_mask;
+                const float add = a.n_dist && apart ? bt[sa_entry(near_d >= a.reach ? a.reach : -a.reach, a.reach, a.causal)] : 0.f;
+                float total = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at_k = 8 * (i >> 2) + 4 * hi + (i & 3), key = k0 + at_k;
+                    float x = S[i] * a.c + add;
+                    if (a.n_dist && !apart) x += bt[sa_entry(qpos - key, a.reach, a.causal)];
+                    float ds = __builtin_amdgcn_exp2f(x - lse) * (dP[i] - delta);
+                    if (edge) {
+                        bool ok = key < sq.lk && (!a.causal || key <= qpos);
+                        if (a.key_mask) ok = ok && km[kb * 32 + at_k] != 0;
+                        ds = ok ? ds : 0.f;
+                    }
+                    S[i] = ds;
+                    total += ds;
+                }
+                if (a.bias_part) {
+                    if (near_d >= a.reach) {
+                        beyond_hi += total;
+                    } else if (far_d <= -a.reach) {
+                        beyond_lo += total;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) skew[(8 * (i >> 2) + 4 * hi + (i & 3)) * 63 + (lane & 31) + 31] = S[i];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        float sum = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) sum += skew[k * 64 + lane];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        // column 31 of the skewed block = query wfirst at key k0
+                        const int dist = wfirst + sq.shift - k0 + lane - 31;
+                        if (dist >= a.reach) beyond_hi += sum;
+                        else if (dist <= -a.reach || (a.causal && dist < 0)) beyond_lo += sum;         // (causal: zeros)
+                        else acc[sa_entry(dist, a.reach, a.causal)] += sum;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = S[8 * ks + j];
+                    bf16x8 P[NP];
+                    sa_planes_f(f, P);
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        bf16x8 A[NP];
+                        sa_cols<NP, DP, KT>(kt, kb * 2 + ks, db, lane, A);
+                        dQ[db] = sa_mma(A, P, dQ[db]);
+                    }
+                }
+            }
+        }
+        if (exists) {
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float x[4] = {dQ[db][i] * a.scale, dQ[db][i + 1] * a.scale, dQ[db][i + 2] * a.scale, dQ[db][i + 3] * a.scale};
+                    sa_store4<NP>(a.dq, (row * a.Hq + h) * a.D, db * 32 + 2 * i + 4 * hi, a.D, x);
+                }
+        }
+    }
+    if (a.bias_part) {
+        // entries of the waves -> one per distance -> buckets, all in fixed order
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { beyond_hi += __shfl_xor(beyond_hi, o); beyond_lo += __shfl_xor(beyond_lo, o); }
+        if (lane == 0) {
+            acc[a.n_dist - 1] += beyond_hi;
+            if (!a.causal) acc[0] += beyond_lo;
+        }
+        __syncthreads();
+        float* acc0 = bt + a.n_dist + NW * SA_SKEW;
+        for (int i = threadIdx.x; i < a.n_dist; i += NT) {
+            float s = acc0[i];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) s += acc0[w * a.n_dist + i];
+            acc0[i] = s;
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < a.n_buckets; t += NT) {
+            float s = 0.f;
+            for (int i = 0; i < a.n_dist; ++i) s += max(0, min(a.buckets[i], a.n_buckets - 1)) == t ? acc0[i] : 0.f;
+            a.bias_part[(static_cast<int64_t>(h) * a.n_buckets + t) * a.bias_slots + static_cast<int64_t>(b) * a.tiles + tile0] = s;
+        }
+    }
+}
+
+// dbias[h, t] = sum of its partials: one workgroup each, strided per thread, then a fixed tree
+__global__ __launch_bounds__(256) void seq_attention_dbias_kernel(const SaK a) {
+    __shared__ double sm[4];
+    const float* p = a.bias_part + static_cast<int64_t>(blockIdx.x) * a.bias_slots;
+    double s = 0.;
+    for (int i = threadIdx.x; i < a.bias_slots; i += 256) s += static_cast<double>(p[i]);
+    s = swr_block_sum_f64<256>(s, sm);
+    if (threadIdx.x == 0) a.dbias[blockIdx.x] = static_cast<float>(s);
+}
+
+template <int NP, int DP, int NW, bool FAST>
+__global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_dkv_kernel(const SaK a) {
+    typedef SaDkv<NP, DP, NW, FAST> Cfg;
+    constexpr int RT = Cfg::RT, RB = RT / 32, NT = NW * 64, KT = NW * 32, TILE = Cfg::TILE;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* rows0 = reinterpret_cast<float*>(smem + Cfg::NBUF * 2 * TILE);      // per buffer: lse of the rows, then delta
+    float* tables = rows0 + Cfg::NBUF * 2 * RT;                                // the group's bias rows
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+
+    int within;
+    const int unit = sa_unit(blockIdx.x, a.per_unit, within);
+    if (unit > a.units) return;
+    if (unit == a.units) {                     // rows of no sequence
+        const int64_t end0 = sa_clamp(a.cu_k[0], 0, a.Tk), beg1 = sa_clamp(a.cu_k[a.B], end0, a.Tk), row = static_cast<int64_t>(a.Hk) * a.D;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, 0, end0, row, NT, within, a.per_unit);
+            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, beg1, a.Tk, row, NT, within, a.per_unit);
+        }
+        return;
+    }
+    const int b = unit / a.Hk, hk = unit % a.Hk;
+    const SaSeq sq = sa_seq(a, b);
+    sa_bias_rows(a, hk * a.G, a.G, tables, NT);
+    for (int64_t tile = within; tile * KT < sq.k_span; tile += a.tiles) {
+        const int first = static_cast<int>(tile * KT), wfirst = first + wave * 32, key = wfirst + (lane & 31);
+        const bool exists = key < sq.k_span;
+        const int64_t row = sq.k0 + (exists ? key : 0);
+        const bool live = key < sq.lk && (!a.key_mask || a.key_mask[row] != 0);
+        const int wlast = min(wfirst + 31, sq.lk - 1);
+        SaRows<NP, DP, FAST, Cfg::LATE> K, V;
+        K.load(a.k, row * a.k_row + hk * a.k_head, live, a.D, a.vk, lane);
+        V.load(a.v, row * a.v_row + hk * a.v_head, live, a.D, a.vv, lane);
+        f32x16 dK[DP / 32], dV[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) { dK[db] = sa_zero16(); dV[db] = sa_zero16(); }
+
+        // queries that see this tile: all of them, or (causal) those at or behind its first key
+        const int q_first = a.causal ? max(0, first - sq.shift) : 0;
+        const int r_begin = q_first / RT, r_end = first < sq.lk ? (sq.lq + RT - 1) / RT : 0, n_r = max(0, r_end - r_begin);
+        const int steps = n_r * a.G;
+        SaStage<NP, DP, RT, NT, FAST> sQ, sD;
+        float ld_l = 0.f, ld_d = 0.f;
+        auto fetch = [&](int step, int buf) {
+            const int h = hk * a.G + step / n_r, q0 = (r_begin + step % n_r) * RT;
+            if (Cfg::DMA) {
+                const sa_lds to = (sa_lds)smem + buf * 2 * TILE;
+                SaDma<DP, RT, NT>::copy(to, a.q, sq.q0, q0, sq.lq, a.q_row, static_cast<int64_t>(h) * a.q_head, a.D, nullptr);
+                SaDma<DP, RT, NT>::copy(to + TILE, a.dout, sq.q0, q0, sq.lq, a.do_row, static_cast<int64_t>(h) * a.do_head, a.D, nullptr);
+            } else {
+                sQ.load(a.q, sq.q0, q0, sq.lq, a.q_row, static_cast<int64_t>(h) * a.q_head, a.D, a.vq, nullptr);
+                sD.load(a.dout, sq.q0, q0, sq.lq, a.do_row, static_cast<int64_t>(h) * a.do_head, a.D, a.vdo, nullptr);
+            }
+            if (threadIdx.x < RT) {
+                const int tok = q0 + threadIdx.x;
+                const int64_t at = static_cast<int64_t>(h) * a.Tq + sq.q0 + tok;
+                ld_l = tok < sq.lq ? a.lse[at] : INFINITY;
+                ld_d = tok < sq.lq ? a.delta[at] : 0.f;
+            }
+        };
+        if (steps > 0) {
+            __syncthreads();
+            if (!Cfg::LATE) fetch(0, 0);
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int q0 = (r_begin + step % n_r) * RT, buf = Cfg::DMA ? step & 1 : 0;
+            const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
+            float *lse_s = rows0 + buf * 2 * RT, *delta_s = lse_s + RT;
+            const float* bt = tables + (step / n_r) * a.n_dist;
+            if (Cfg::LATE) fetch(step, 0);
+            if (!Cfg::DMA) {
+                if (step > 0) __syncthreads();
+                sQ.store(qt);
+                sD.store(dt);
+            }
+            if (threadIdx.x < RT) { lse_s[threadIdx.x] = ld_l; delta_s[threadIdx.x] = ld_d; }
+            if (Cfg::DMA) sa_dma_wait();
+            __syncthreads();
+            if (!Cfg::LATE && step + 1 < steps) fetch(step + 1, buf ^ 1);
+            if (wfirst > wlast) continue;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int r0 = q0 + rb * 32, rlast = min(r0 + 31, sq.lq - 1);
+                if (r0 >= sq.lq || (a.causal && rlast + sq.shift < wfirst)) continue;
+                f32x16 S = sa_zero16(), dP = sa_zero16();
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                    bf16x8 A[NP], B[NP];
+                    sa_rows<NP, DP, RT>(qt, rb, s, lane, A);
+                    K.get(s, B);
+                    S = sa_mma(A, B, S);
+                    sa_rows<NP, DP, RT>(dt, rb, s, lane, A);
+                    V.get(s, B);
+                    dP = sa_mma(A, B, dP);
+                }
+                const int near_d = r0 + sq.shift - wlast, far_d = rlast + sq.shift - wfirst;
+                const bool apart = near_d >= a.reach || far_d <= -a.reach;
+                const float add = a.n_dist && apart ? bt[sa_entry(near_d >= a.reach ? a.reach : -a.reach, a.reach, a.causal)] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at_r = rb * 32 + 8 * (i >> 2) + 4 * hi + (i & 3), dist = q0 + at_r + sq.shift - key;
+                    float x = S[i] * a.c + add;
+                    if (a.n_dist && !apart) x += bt[sa_entry(dist, a.reach, a.causal)];
+                    const bool ok = live && (!a.causal || dist >= 0);
+                    const float p = __builtin_amdgcn_exp2f(x - lse_s[at_r]);
+                    S[i] = ok ? p : 0.f;
+                    dP[i] = ok ? p * (dP[i] - delta_s[at_r]) : 0.f;
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = S[8 * ks + j];
+                    bf16x8 P[NP], A[NP];
+                    sa_planes_f(f, P);
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        sa_cols<NP, DP, RT>(dt, rb * 2 + ks, db, lane, A);
+                        dV[db] = sa_mma(A, P, dV[db]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = dP[8 * ks + j];
+                    sa_planes_f(f, P);
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        sa_cols<NP, DP, RT>(qt, rb * 2 + ks, db, lane, A);
+                        dK[db] = sa_mma(A, P, dK[db]);
+                    }
+                }
+            }
+        }
+        if (exists) {
+            const int64_t o = (row * a.Hk + hk) * a.D;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = db * 32 + 2 * i + 4 * hi;
+                    const float x[4] = {dK[db][i] * a.scale, dK[db][i + 1] * a.scale, dK[db][i + 2] * a.scale, dK[db][i + 3] * a.scale};
+                    const float y[4] = {dV[db][i], dV[db][i + 1], dV[db][i + 2], dV[db][i + 3]};
+                    sa_store4<NP>(a.dk, o, d, a.D, x);
+                    sa_store4<NP>(a.dv, o, d, a.D, y);
+                }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------- host
+struct SaBwdPlan {
+    SaK q, kv;
+    int nw_q, nw_kv;
+    size_t delta, bytes;
+    bool fits;
+};
+static SaBwdPlan sa_bwd_plan(const swr_seq_attention_args* p) {
+    SaBwdPlan pl{};
+    pl.q = pl.kv = sa_args(p);
+    pl.nw_q = sa_waves(p->max_q, pl.q, p->dtype == SWR_F32);
+    pl.nw_kv = sa_waves(p->max_k, pl.kv, p->dtype == SWR_F32);
+    pl.q.tiles = static_cast<int>(std::max<int64_t>(1, swr_ceil_div(p->max_q, pl.nw_q * 32)));
+    pl.kv.tiles = static_cast<int>(std::max<int64_t>(1, swr_ceil_div(p->max_k, pl.nw_kv * 32)));
+    pl.q.per_unit = pl.q.tiles * pl.q.G;
+    pl.kv.per_unit = pl.kv.tiles;
+    pl.fits = sa_grid(pl.q) && sa_grid(pl.kv);
+    const int64_t slots = static_cast<int64_t>(p->B) * pl.q.tiles;
+    pl.q.bias_slots = static_cast<int>(slots);
+    pl.delta = static_cast<size_t>(p->Hq) * p->Tq * sizeof(float);
+    pl.bytes = pl.delta + (p->dbias && p->n_dist ? static_cast<size_t>(p->Hq) * p->n_buckets * slots * sizeof(float) : 0) + 256;
+    return pl;
+}
+
+extern "C" size_t swr_seq_attention_bwd_workspace_bytes(const swr_seq_attention_args* p) {
+    return sa_check(p, true) == SWR_OK ? sa_bwd_plan(p).bytes : 0;
+}
+
+template <int NP, int DP, int NW, bool FAST>
+static int sa_dq_launch(SaK& a, hipStream_t st) {
+    const int lds = SaDq<NP, DP, NW, FAST>::lds(a);
+    SWR_REQUIRE(lds <= 160 * 1024, SWR_ERR_UNSUPPORTED);
+    if (lds > 64 * 1024 && !swr_raise_lds(reinterpret_cast<const void*>(seq_attention_dq_kernel<NP, DP, NW, FAST>), 160 * 1024)) return SWR_ERR_LAUNCH;
+    hipLaunchKernelGGL((seq_attention_dq_kernel<NP, DP, NW, FAST>), dim3(sa_grid(a)), dim3(NW * 64), lds, st, a);
+    return SWR_OK;
+}
+template <int NP, int DP, int NW, bool FAST>
+static int sa_dkv_launch(SaK& a, hipStream_t st) {
+    const int lds = SaDkv<NP, DP, NW, FAST>::lds(a);
+    SWR_REQUIRE(lds <= 160 * 1024, SWR_ERR_UNSUPPORTED);
+    if (lds > 64 * 1024 && !swr_raise_lds(reinterpret_cast<const void*>(seq_attention_dkv_kernel<NP, DP, NW, FAST>), 160 * 1024)) return SWR_ERR_LAUNCH;
+    hipLaunchKernelGGL((seq_attention_dkv_kernel<NP, DP, NW, FAST>), dim3(sa_grid(a)), dim3(NW * 64), lds, st, a);
+    return SWR_OK;
+}
+template <int NP, int DP>
+static int sa_bwd_dp(SaBwdPlan& pl, hipStream_t st) {
+    SaK &q = pl.q, &kv = pl.kv;
+    if (!q.fast) {
+        const int rc = sa_dq_launch<NP, DP, 4, false>(q, st);
+        return rc != SWR_OK ? rc : sa_dkv_launch<NP, DP, 4, false>(kv, st);
+    }
+    if constexpr (NP * DP >= 384) {
+        const int rc = sa_dq_launch<NP, DP, 4, true>(q, st);
+        return rc != SWR_OK ? rc : sa_dkv_launch<NP, DP, 4, true>(kv, st);
+    } else {
+        const int rc = pl.nw_q == 1 ? sa_dq_launch<NP, DP, 1, true>(q, st)
+                                    : (pl.nw_q == 2 ? sa_dq_launch<NP, DP, 2, true>(q, st) : sa_dq_launch<NP, DP, 4, true>(q, st));
+        if (rc != SWR_OK) return rc;
+        return pl.nw_kv == 1 ? sa_dkv_launch<NP, DP, 1, true>(kv, st)
+                             : (pl.nw_kv == 2 ? sa_dkv_launch<NP, DP, 2, true>(kv, st) : sa_dkv_launch<NP, DP, 4, true>(kv, st));
+    }
+}
+
+extern "C" int swr_seq_attention_bwd(const swr_seq_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = sa_check(p, true);
+    if (rc != SWR_OK) return rc;
+    SaBwdPlan pl = sa_bwd_plan(p);
+    SWR_REQUIRE(pl.fits, SWR_ERR_UNSUPPORTED);
+    SWR_REQUIRE(workspace && workspace_bytes >= pl.bytes, SWR_ERR_WORKSPACE);
+    SWR_REQUIRE(swr_aligned16(workspace), SWR_ERR_ALIGN);
+    SaK &q = pl.q, &kv = pl.kv;
+    q.delta = kv.delta = static_cast<float*>(workspace);
+    if (p->dbias && p->n_dist) q.bias_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (pl.delta + 255) / 256 * 256);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int r = p->dtype == SWR_F32 ? (p->D <= 32 ? sa_bwd_dp<3, 32>(pl, st) : (p->D <= 64 ? sa_bwd_dp<3, 64>(pl, st) : sa_bwd_dp<3, 128>(pl, st)))
+                                      : (p->D <= 32 ? sa_bwd_dp<1, 32>(pl, st) : (p->D <= 64 ? sa_bwd_dp<1, 64>(pl, st) : sa_bwd_dp<1, 128>(pl, st)));
+    if (r != SWR_OK) return r;
+    if (q.bias_part) hipLaunchKernelGGL(seq_attention_dbias_kernel, dim3(static_cast<unsigned>(p->Hq) * p->n_buckets), dim3(256), 0, st, q);
+    return swr_launch_status();
+}

@@ -154,6 +154,32 @@ class LayerNormArgs(C.Structure):
                 ("dbeta", C.c_void_p)]
 
 
+class SeqAttentionArgs(C.Structure):
+    _fields_ = [("Tq", C.c_int64), ("Tk", C.c_int64), ("B", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
+                ("dtype", C.c_int32), ("causal", C.c_int32), ("max_q", C.c_int32), ("max_k", C.c_int32), ("scale", C.c_float),
+                ("n_dist", C.c_int32), ("n_buckets", C.c_int32), ("pad", C.c_int32),
+                ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("k", C.c_void_p), ("k_row", C.c_int64), ("k_head", C.c_int64),
+                ("v", C.c_void_p), ("v_row", C.c_int64), ("v_head", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_len", C.c_void_p), ("k_len", C.c_void_p),
+                ("key_mask", C.c_void_p), ("bias", C.c_void_p), ("buckets", C.c_void_p),
+                ("dout", C.c_void_p), ("do_row", C.c_int64), ("do_head", C.c_int64),
+                ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dbias", C.c_void_p), ("err_flag", C.c_void_p)]
+
+
+SEQ_MAX_DIM, SEQ_MAX_DIST, SEQ_MAX_BUCKETS, SEQ_MAX_TABLE = 128, 4097, 256, 8192        # SWR_SEQ_MAX_*
+
+
+class NormGateArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float), ("scale", C.c_float),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64), ("gate", C.c_void_p),
+                ("ldg", C.c_int64), ("w_post", C.c_void_p), ("w_pre", C.c_void_p), ("z", C.c_void_p), ("u", C.c_void_p),
+                ("ry", C.c_void_p), ("rz", C.c_void_p), ("dz", C.c_void_p), ("lddz", C.c_int64), ("du", C.c_void_p),
+                ("lddu", C.c_int64), ("dx", C.c_void_p), ("dy", C.c_void_p), ("dgate", C.c_void_p), ("dw_post", C.c_void_p),
+                ("dw_pre", C.c_void_p)]
+
+
+NORM_GATE_MAX_WIDTH = 8192         # SWR_NORM_GATE_MAX_WIDTH
 ADAM_MAX_TABLES = 16        # SWR_ADAM_MAX_TABLES
 
 
@@ -302,6 +328,13 @@ _SIGS = {
     "swr_star_layers_bwd": (C.c_int, [_P, _I, _P]),
     "swr_eval_metrics_workspace_bytes": (_Z, [_L, _I]),
     "swr_eval_metrics": (C.c_int, [_P, _P, _I, _P, _I, _L, _I, _P, _P, _P, _Z, _P]),
+    "swr_seq_attention_fwd_workspace_bytes": (_Z, [_P]),
+    "swr_seq_attention_fwd": (C.c_int, [_P, _P, _Z, _P]),
+    "swr_seq_attention_bwd_workspace_bytes": (_Z, [_P]),
+    "swr_seq_attention_bwd": (C.c_int, [_P, _P, _Z, _P]),
+    "swr_norm_gate_fwd": (C.c_int, [_P, _P]),
+    "swr_norm_gate_bwd_workspace_bytes": (_Z, [_L, _I]),
+    "swr_norm_gate_bwd": (C.c_int, [_P, _P, _Z, _P]),
     "swr_dp_finish": (C.c_int, [_P, _L, _L, _P, _P, _L, _P, _I, _I, _F, _P]),
 }
 EXPORTS = tuple(_SIGS)

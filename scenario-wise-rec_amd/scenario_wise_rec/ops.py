@@ -2694,3 +2694,269 @@ class BlockSelect(Function):
 
 def block_select(V, domain, D, Hh):
     return BlockSelect.apply(V, domain, int(D), int(Hh))
+
+
+# =========================================================================== attention over histories, norms around a block
+_SEQ_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _on_device_of(t):
+    """The launches go to the current stream of t's device, whichever device is current."""
+    return torch.cuda.device(t.device)
+
+
+def _unit_last(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def seq_buckets(n_buckets, max_distance, causal=True, device="cuda"):
+    """The distance -> bucket table of a relative position bias (`seq_attention(buckets=...)`), int32.
+
+    One-sided (causal): distances 0 .. max_distance, further ones share the last entry.  The first half of the buckets hold one
+    distance each, the others grow in equal ratios up to max_distance.  Both ways: entries -max_distance .. max_distance, half of the
+    buckets (n_buckets even) for each sign.  The borders are compared in whole numbers."""
+    side = n_buckets if causal else n_buckets // 2
+    half = side // 2
+    if n_buckets < 1 or side < 2 or (not causal and n_buckets % 2) or n_buckets > H.SEQ_MAX_BUCKETS:
+        raise ValueError(f"seq_buckets: n_buckets = {n_buckets} (2 .. {H.SEQ_MAX_BUCKETS}; even and at least 4 when not causal)")
+    if max_distance <= half or (max_distance if causal else 2 * max_distance) >= H.SEQ_MAX_DIST:
+        raise ValueError(f"seq_buckets: max_distance = {max_distance} out of range for {n_buckets} buckets")
+    # bucket half + t starts at the smallest r with r >= half (max_distance / half)^(t / (side - half))
+    one, t, m = [], 0, side - half
+    for r in range(max_distance + 1):
+        if r < half:
+            one.append(r)
+            continue
+        while t + 1 < m and r ** m * half ** (t + 1) >= max_distance ** (t + 1) * half ** m:
+            t += 1
+        one.append(half + t)
+    table = one if causal else [one[-r] + side for r in range(-max_distance, 0)] + one
+    return torch.tensor(table, dtype=torch.int32, device=device)
+
+
+def _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets):
+    a = H.SeqAttentionArgs()
+    a.Tq, a.Tk, a.B, a.Hq, a.Hk, a.D = q.shape[0], k.shape[0], cu_q.numel() - 1, q.shape[1], k.shape[1], q.shape[2]
+    a.dtype, a.causal, a.max_q, a.max_k, a.scale = H.dtype_code(q), int(meta["causal"]), meta["max_q"], meta["max_k"], meta["scale"]
+    a.q, a.q_row, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.k_row, a.k_head = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_row, a.v_head = v.data_ptr(), v.stride(0), v.stride(1)
+    a.out, a.cu_q, a.cu_k = out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if q_len is not None:
+        a.q_len = q_len.data_ptr()
+    if k_len is not None:
+        a.k_len = k_len.data_ptr()
+    if key_mask is not None:
+        a.key_mask = key_mask.data_ptr()
+    if bias is not None:
+        a.n_dist, a.n_buckets, a.bias, a.buckets = buckets.numel(), bias.shape[1], bias.data_ptr(), buckets.data_ptr()
+    a.err_flag = H.err_flag(q.device).data_ptr()
+    return a
+
+
+class SeqAttention(Function):
+    """csrc/seq_attention_fwd.hip / seq_attention_bwd.hip; arguments checked by `seq_attention`."""
+
+    @staticmethod
+    def forward(ctx, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
+        ctx.meta = meta
+        if q.numel() == 0 or k.numel() == 0:                       # no query, or no key that any query could see
+            ctx.save_for_backward(q, k, v, bias)
+            return q.new_zeros(q.shape)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        want = any(ctx.needs_input_grad[1:5])
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
+        a = _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
+        with _on_device_of(q):
+            nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            H.check(lib.swr_seq_attention_fwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_seq_attention_fwd")
+        ctx.save_for_backward(q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        if len(ctx.saved_tensors) == 4:
+            return (None,) + tuple(torch.zeros_like(t) if t is not None and n else None
+                                   for t, n in zip(ctx.saved_tensors, ctx.needs_input_grad[1:5])) + (None,) * 6
+        q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets = ctx.saved_tensors
+        dev = q.device
+        dout = _unit_last(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[4] else None
+        a = _seq_args(ctx.meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
+        a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        if dbias is not None:
+            a.dbias = dbias.data_ptr()
+        with _on_device_of(q):
+            nbytes = lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            H.check(lib.swr_seq_attention_bwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_seq_attention_bwd")
+        need = ctx.needs_input_grad
+        return None, dq if need[1] else None, dk if need[2] else None, dv if need[3] else None, dbias, None, None, None, None, None, None
+
+
+def _index_vector(t, name, n, device):
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.numel() != n):
+        raise ValueError(f"seq_attention: {name} must be int32 of shape ({'sequences + 1' if n is None else n},), got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise H.SwrError(f"seq_attention: {name} is on {t.device}, the queries on {device}")
+    return t.contiguous()
+
+
+def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True, scale=None, bias=None, buckets=None,
+                  key_mask=None, q_len=None, k_len=None):
+    """Self-attention over packed sequences: softmax(scale q k^T + bias) v of every sequence, [Tq, Hq, D] in q's dtype.
+
+    q [Tq, Hq, D], k / v [Tk, Hk, D]: fp32 or bf16, D <= 128, any row and head strides; query head h reads key head h // (Hq // Hk).
+    cu_q / cu_k (int32, [sequences + 1]): prefix sums of the sequences' rows, cu_k = cu_q when left out.  q_len / k_len (int32,
+    [sequences], optional): rows in use of each (a padded batch; a cache with room behind it); with cu_k left out k_len = q_len.
+    causal: query i of a sequence sees its keys j <= i + (keys - queries) -- the last query stands at the last key, so one call serves
+    training, a whole prompt, and a few new tokens over cached keys.  key_mask (bool / uint8, [Tk]): 0 hides a key from every query.
+    bias (fp32, [Hq, n_buckets]) with buckets (`seq_buckets`): a learned bias per head and bucket of the distance i + (keys - queries) - j.
+    max_q / max_k: the longest sequence if known on the host (chooses the launch and its tiling, right for any value; default: all rows).
+
+    A row without a visible key, and rows of no sequence or beyond q_len, are zeros with zero gradients; keys beyond k_len or hidden
+    by key_mask may hold anything.  Differentiable in q, k, v and bias, deterministic.  Bad prefix sums, lengths and bucket ids are
+    clamped and raise IndexError at the next `_hip.check_errors()`."""
+    H.require_device(q, k, v, cu_q, bias)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"seq_attention: q [Tq, Hq, D], k and v [Tk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _SEQ_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise H.SwrError(f"seq_attention: q, k, v must all be float32 or all bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.device != q.device or v.device != q.device:
+        raise H.SwrError("seq_attention: q, k, v are on different devices")
+    Hq, Hk, D = q.shape[1], k.shape[1], q.shape[2]
+    if not 1 <= D <= H.SEQ_MAX_DIM or Hk < 1 or Hq % Hk or Hq < Hk:
+        raise ValueError(f"seq_attention: head width {D} (at most {H.SEQ_MAX_DIM}) and {Hq} query heads over {Hk} key heads")
+    cu_q = _index_vector(cu_q, "cu_q", None, q.device)
+    n = cu_q.numel() - 1
+    if n < 0:
+        raise ValueError("seq_attention: cu_q needs at least one entry")
+    if cu_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError("seq_attention: cu_k is needed where keys and queries differ in rows")
+        cu_k = cu_q
+        k_len = q_len if k_len is None else k_len
+        max_k = max_q if max_k is None else max_k
+    else:
+        cu_k = _index_vector(cu_k, "cu_k", n + 1, q.device)
+    q_len = None if q_len is None else _index_vector(q_len, "q_len", n, q.device)
+    k_len = None if k_len is None else _index_vector(k_len, "k_len", n, q.device)
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (k.shape[0],) or key_mask.device != q.device:
+            raise ValueError(f"seq_attention: key_mask must be bool or uint8 of shape ({k.shape[0]},) on {q.device}")
+        key_mask = key_mask.contiguous()
+    if (bias is None) != (buckets is None):
+        raise ValueError("seq_attention: bias and buckets come together")
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.dim() != 2 or bias.shape[0] != Hq or not 1 <= bias.shape[1] <= H.SEQ_MAX_BUCKETS:
+            raise ValueError(f"seq_attention: bias must be float32 [{Hq}, n_buckets <= {H.SEQ_MAX_BUCKETS}], got {bias.dtype} {tuple(bias.shape)}")
+        buckets = _index_vector(buckets, "buckets", buckets.numel(), q.device)
+        if not 1 <= buckets.numel() <= H.SEQ_MAX_DIST or (not causal and buckets.numel() % 2 == 0):
+            raise ValueError(f"seq_attention: {buckets.numel()} bucket entries (at most {H.SEQ_MAX_DIST}, odd when not causal)")
+        if buckets.numel() * (Hq // Hk) > H.SEQ_MAX_TABLE:
+            raise ValueError(f"seq_attention: {buckets.numel()} bucket entries x {Hq // Hk} heads of a group (at most {H.SEQ_MAX_TABLE})")
+        bias = bias.contiguous()
+    meta = {"causal": bool(causal), "scale": float(D ** -0.5 if scale is None else scale),
+            "max_q": q.shape[0] if max_q is None else min(int(max_q), q.shape[0]),
+            "max_k": k.shape[0] if max_k is None else min(int(max_k), k.shape[0])}
+    return SeqAttention.apply(meta, _unit_last(q), _unit_last(k), _unit_last(v), bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+
+
+def _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz):
+    a = H.NormGateArgs()
+    a.M, a.N, a.dtype, a.eps, a.scale = x.shape[0], x.shape[1], H.dtype_code(x), meta["eps"], meta["scale"]
+    a.x, a.ldx = x.data_ptr(), x.stride(0)
+    if y is not None:
+        a.y, a.ldy = y.data_ptr(), y.stride(0)
+    if gate is not None:
+        a.gate, a.ldg = gate.data_ptr(), gate.stride(0)
+    for name, t in (("w_post", w_post), ("w_pre", w_pre), ("ry", ry), ("rz", rz)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    return a
+
+
+class NormGateResidual(Function):
+    """csrc/norm_gate.hip; arguments checked by `norm_gate_residual`.  Returns (z or None, u or None)."""
+
+    @staticmethod
+    def forward(ctx, meta, x, y, gate, w_post, w_pre):
+        ctx.set_materialize_grads(False)
+        dev, M = x.device, x.shape[0]
+        z = torch.empty(x.shape, dtype=x.dtype, device=dev) if y is not None else None
+        u = torch.empty(x.shape, dtype=x.dtype, device=dev) if w_pre is not None else None
+        want = any(ctx.needs_input_grad)
+        stat = lambda w: torch.empty(M, dtype=torch.float32, device=dev) if want and w is not None else None
+        ry, rz = stat(w_post), stat(w_pre)
+        a = _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz)
+        a.z, a.u = (None if z is None else z.data_ptr()), (None if u is None else u.data_ptr())
+        with _on_device_of(x):
+            if M:
+                H.check(lib.swr_norm_gate_fwd(C.byref(a), H.stream()), "swr_norm_gate_fwd")
+        ctx.meta = meta
+        ctx.save_for_backward(x, y, gate, w_post, w_pre, ry, rz)
+        return z, u
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dz, du):
+        x, y, gate, w_post, w_pre, ry, rz = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dz is None and du is None:
+            return (None,) * 6
+        if x.numel() == 0:
+            return (None,) + tuple(torch.zeros_like(t) if t is not None and n else None for t, n in zip((x, y, gate, w_post, w_pre), need[1:]))
+        dev, M, N = x.device, x.shape[0], x.shape[1]
+        empty = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+        dx, dy, dg = empty(x), empty(y), empty(gate)
+        dwp, dwn = empty(w_post) if need[4] else None, empty(w_pre) if need[5] else None
+        a = _norm_gate_args(ctx.meta, x, y, gate, w_post, w_pre, ry, rz)
+        if dz is not None:
+            dz = _unit_last(dz if dz.dtype == x.dtype else dz.to(x.dtype))
+            a.dz, a.lddz = dz.data_ptr(), dz.stride(0)
+        if du is not None:
+            du = _unit_last(du if du.dtype == x.dtype else du.to(x.dtype))
+            a.du, a.lddu = du.data_ptr(), du.stride(0)
+        a.dx = dx.data_ptr()
+        for name, t in (("dy", dy), ("dgate", dg), ("dw_post", dwp), ("dw_pre", dwn)):
+            if t is not None:
+                setattr(a, name, t.data_ptr())
+        with _on_device_of(x):
+            nbytes = lib.swr_norm_gate_bwd_workspace_bytes(M, N) if dwp is not None or dwn is not None else 0
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            H.check(lib.swr_norm_gate_bwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_norm_gate_bwd")
+        return None, dx if need[1] else None, dy if need[2] else None, dg if need[3] else None, dwp, dwn
+
+
+def norm_gate_residual(x, y=None, gate=None, w_post=None, w_pre=None, scale=1.0, eps=1e-6):
+    """The norms behind one block and before the next, fused with the block's gate and residual:
+
+        t = y rms(y) w_post (w_post None: y),  z = x + scale sigmoid(gate) t (gate None: no sigmoid),  u = z rms(z) w_pre
+
+    x (the residual stream), y (the block's output), gate (logits, e.g. `GateNU.logits`): [M, N], all fp32 or all bf16, rows may be
+    strided; w_post, w_pre: fp32 [N]; rms(a) = (mean a^2 + eps)^-1/2.  Returns z, or (z, u) with w_pre, or u alone with w_pre and
+    without y (the norm before the first block).  Sums in fp32; u and the gradients start from the unrounded z."""
+    H.require_device(x, y, gate, w_post, w_pre)
+    if x.dim() != 2 or x.shape[1] < 1 or x.shape[1] > H.NORM_GATE_MAX_WIDTH:
+        raise ValueError(f"norm_gate_residual: x must be [M, N <= {H.NORM_GATE_MAX_WIDTH}], got {tuple(x.shape)}")
+    if x.dtype not in _SEQ_TYPES:
+        raise H.SwrError(f"norm_gate_residual: float32 or bfloat16, got {x.dtype}")
+    if y is None and (w_pre is None or gate is not None or w_post is not None):
+        raise ValueError("norm_gate_residual: without y only the norm of x (w_pre) is left")
+    for name, t in (("y", y), ("gate", gate)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"norm_gate_residual: {name} must match x ({tuple(x.shape)}, {x.dtype}), got {tuple(t.shape)}, {t.dtype}, {t.device}")
+    for name, t in (("w_post", w_post), ("w_pre", w_pre)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (x.shape[1],) or t.device != x.device):
+            raise ValueError(f"norm_gate_residual: {name} must be float32 [{x.shape[1]}] on {x.device}, got {t.dtype} {tuple(t.shape)}")
+    flat = lambda t: None if t is None else _unit_last(t)
+    meta = {"scale": float(scale), "eps": float(eps)}
+    z, u = NormGateResidual.apply(meta, flat(x), flat(y), flat(gate), None if w_post is None else w_post.contiguous(),
+                                  None if w_pre is None else w_pre.contiguous())
+    return u if y is None else (z if w_pre is None else (z, u))
