@@ -28,7 +28,7 @@ struct SaK {
     int B, Hq, Hk, G, D, causal;
     float c;                               // scale * log2(e)
     float scale;
-    int n_dist, n_buckets, reach;          // reach: largest |distance| with an entry of its own
+    int n_dist, n_buckets, reach, row;     // reach: largest |distance| with an entry of its own; row: sa_row_entries
     int vq, vk, vv, vo, vdo;               // elements per load of q, k, v, out, dout rows: 8, 4 or 1
     bool fast;                             // all of them 8, row strides below 2^23 elements (64 rows within 32-bit byte offsets)
     const void *q, *k, *v; int64_t q_row, q_head, k_row, k_head, v_row, v_head;
@@ -134,7 +134,9 @@ struct SaStage {
     // rows first .. first + R - 1 of a sequence whose row 0 is `row0`; rows >= limit (limit > first) or masked read as zeros
     __device__ __forceinline__ void load(const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D, int vw,
                                          const uint8_t* mask) {
-        const int chunk = threadIdx.x % CPR, row = threadIdx.x / CPR;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));          // (addresses are made here, not kept in registers across the tile loop)
+        const int chunk = tid % CPR, row = tid / CPR;
         const T* p = static_cast<const T*>(base) + (row0 + first) * stride + head_off;
         keep = 0;
 #pragma unroll
@@ -152,7 +154,9 @@ struct SaStage {
         }
     }
     __device__ __forceinline__ void store(sa_lds dst) const {
-        const int chunk = threadIdx.x % CPR, row = threadIdx.x / CPR;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int chunk = tid % CPR, row = tid / CPR;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             SaRaw<NP> x = r[i];
@@ -181,7 +185,9 @@ struct SaDma {
     static_assert(R * CPR % NT == 0 && NT % CPR == 0, "whole chunks per thread");
     static __device__ __forceinline__ void copy(sa_lds dst, const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D,
                                                 const uint8_t* mask) {
-        const int slot = threadIdx.x % CPR, row = threadIdx.x / CPR;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int slot = tid % CPR, row = tid / CPR;
         const uint16_t* p = static_cast<const uint16_t*>(base) + (row0 + first) * stride + head_off;
         const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)) + (threadIdx.x & ~63u) * 16);
 #pragma unroll
@@ -195,26 +201,35 @@ struct SaDma {
     }
 };
 
-// left operand of a product over the columns: row (lane & 31) of block rb, columns 16 s + 8 hi .. + 7
+// What a lane reads of a tile.  Both readers' byte offsets are a lane constant XOR a compile-time constant (the swizzle only sees the
+// low row bits), so one instruction makes an address; `fresh` keeps the compiler from hoisting dozens of them out of the tile loop
+// into registers.
 template <int NP, int DP, int R>
-__device__ __forceinline__ void sa_rows(sa_lds tile, int rb, int s, int lane, bf16x8 (&o)[NP]) {
-    const int off = sa_off<DP>(rb * 32 + (lane & 31), 2 * s + (lane >> 5));
-#pragma unroll
-    for (int pl = 0; pl < NP; ++pl) o[pl] = *reinterpret_cast<sa_lds_v>(tile + pl * (R * DP * 2) + off);
-}
-// left operand of a product over the rows: column 32 db + (lane & 31), rows 16 ks + {4 hi + 0..3, 8 + 4 hi + 0..3}
-template <int NP, int DP, int R>
-__device__ __forceinline__ void sa_cols(sa_lds tile, int ks, int db, int lane, bf16x8 (&o)[NP]) {
-    const int row = 16 * ks + 4 * (lane >> 5) + ((lane >> 2) & 3);
-    const int chunk = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), half = (lane & 1) * 8;
-    const int o0 = sa_off<DP>(row, chunk) + half, o1 = sa_off<DP>(row + 8, chunk) + half;
-#pragma unroll
-    for (int pl = 0; pl < NP; ++pl) {
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(tile + pl * (R * DP * 2) + o0));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(tile + pl * (R * DP * 2) + o1));
-        o[pl] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+struct SaLane {
+    int row, col;
+    __device__ __forceinline__ SaLane(int lane) {
+        row = sa_off<DP>(lane & 31, lane >> 5);
+        const int chunk = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
+        col = sa_off<DP>(4 * (lane >> 5) + ((lane >> 2) & 3), chunk) + (lane & 1) * 8;
     }
-}
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(row), "+v"(col)); }
+    // left operand of a product over the columns: row (lane & 31) of block rb, columns 16 s + 8 hi .. + 7
+    __device__ __forceinline__ void rows(sa_lds tile, int rb, int s, bf16x8 (&o)[NP]) const {
+        const sa_lds p = tile + rb * (32 * DP * 2) + (row ^ (s << 5));
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) o[pl] = *reinterpret_cast<sa_lds_v>(p + pl * (R * DP * 2));
+    }
+    // left operand of a product over the rows: column 32 db + (lane & 31), rows 16 ks + {4 hi + 0..3, 8 + 4 hi + 0..3}
+    __device__ __forceinline__ void cols(sa_lds tile, int ks, int db, bf16x8 (&o)[NP]) const {
+        const sa_lds p0 = tile + ks * (16 * DP * 2) + (col ^ (db << 6)), p1 = tile + ks * (16 * DP * 2) + 8 * DP * 2 + (col ^ (db << 6) ^ (2 << 4));
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(p0 + pl * (R * DP * 2)));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(reinterpret_cast<sa_lds_tr>(p1 + pl * (R * DP * 2)));
+            o[pl] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
 // right operand held in registers: row `off` (elements) of a matrix, columns 16 s + 8 hi .. + 7 (zeros beyond D or where !ok)
 // (FAST: `off` has to be a valid row where !ok, too)
 template <int NP, bool FAST>
@@ -295,15 +310,44 @@ __device__ __forceinline__ int sa_unit(int id, int per_unit, int& within) {
     return (slot / per_unit) * 8 + (id & 7);
 }
 
-// entry of the distance table, clamped to its reach (causal: distances 0 .. reach, else -reach .. reach)
-__device__ __forceinline__ int sa_entry(int dist, int reach, int causal) {
-    return causal ? max(0, min(dist, reach)) : max(-reach, min(dist, reach)) + reach;
+// Position bias in LDS: one row per head, entry (distance + SA_PAD), with the table's ends repeated and, causal, -inf below distance
+// 0 (which masks): a 32 x 32 block that touches the table reads it at one base per lane and constant offsets, without a clamp or a
+// comparison.  Blocks wholly beyond the reach take one value.  Without a bias the row is that of a one-entry table of 0, both ways none.
+#define SA_PAD 64
+__host__ __device__ __forceinline__ int sa_row_entries(int n_dist, int reach, int causal) {
+    return (n_dist || causal) ? (causal ? reach : 2 * reach) + 2 * SA_PAD + 1 : 0;
 }
 // bias in the exponent's base-2 unit; a finite value stays finite (a bias of the type's lowest value masks relative to the row's
 // other scores, it does not empty the row)
 __device__ __forceinline__ float sa_bias2(float b) {
     const float x = b * SA_LOG2E;
     return (__builtin_isinf(x) && !__builtin_isinf(b)) ? copysignf(3.402823466e38f, x) : x;
+}
+__device__ __forceinline__ int sa_bucket(const SaK& a, int i) { return max(0, min(a.buckets[i], a.n_buckets - 1)); }
+// rows of heads h .. h + heads - 1
+__device__ __forceinline__ void sa_bias_rows(const SaK& a, int h, int heads, float* rows, int nthreads) {
+    const int low = a.causal ? 0 : -a.reach;
+    for (int i = threadIdx.x; i < heads * a.row; i += nthreads) {
+        const int d = i % a.row - SA_PAD + low;
+        float x = 0.f;
+        if (a.n_dist) x = sa_bias2(a.bias[static_cast<int64_t>(h + i / a.row) * a.n_buckets + sa_bucket(a, max(low, min(d, a.reach)) - low)]);
+        rows[i] = a.causal && d < 0 ? -INFINITY : x;
+    }
+}
+// what a block whose distances span near .. far needs: 0 = one value (at .x of the row), 1 = the row
+struct SaSpan { bool apart; int entry; };
+__device__ __forceinline__ SaSpan sa_span(const SaK& a, int near_d, int far_d) {
+    SaSpan s;
+    const bool hi = near_d >= a.reach, lo = !a.causal && far_d <= -a.reach;
+    s.apart = a.row == 0 || hi || lo;
+    s.entry = hi ? (a.causal ? a.reach : 2 * a.reach) + SA_PAD : SA_PAD;
+    return s;
+}
+// entry of distance d
+__device__ __forceinline__ int sa_entry(const SaK& a, int d) { return d + SA_PAD + (a.causal ? 0 : a.reach); }
+// hidden key of result row i (km: the block's flags from row 4 hi on, 4-byte aligned)
+__device__ __forceinline__ bool sa_masked(const uint8_t* km, int i) {
+    return ((*reinterpret_cast<const uint32_t*>(km + 8 * (i >> 2)) >> (8 * (i & 3))) & 0xff) == 0;
 }
 // rows outside every sequence (before the first, behind the last) are zeros in every output
 __device__ __forceinline__ void sa_zero_rows(void* base, int elem, int64_t r0, int64_t r1, int64_t row_elems, int nthreads, int part, int parts) {

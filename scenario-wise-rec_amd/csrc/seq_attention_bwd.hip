@@ -20,8 +20,8 @@ int sa_waves(int64_t columns, const SaK& a, bool fp32);
 unsigned sa_grid(SaK& a);
 
 // waves per SIMD the registers are bounded for (512 / waves each)
-#define SA_WAVES_DQ(NP, DP) ((NP) * (DP) >= 128 ? 1 : 2)
-#define SA_WAVES_DKV(NP, DP) ((NP) * (DP) >= 128 ? 1 : 2)
+#define SA_WAVES_DQ(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : 2)
+#define SA_WAVES_DKV(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : ((NP) * (DP) == 32 ? 3 : 2))
 #define SA_SKEW 2048                           // floats of a wave's skewed 32 x 32 block (32 rows of 64)
 
 // dq: DMA and buffers as in the forward; 32 keys a step at DP = 128, so that two workgroups fit a CU's LDS beside the skew blocks
@@ -30,31 +30,30 @@ struct SaDq {
     static constexpr bool DMA = FAST && NP == 1;
     static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr int TILE = NP * KT * DP * 2;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.n_dist + (a.bias_part ? NW * (SA_SKEW + a.n_dist) : 0)) * 4; }
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.row + (a.bias_part ? NW * (SA_SKEW + a.n_dist) + a.n_dist : 0)) * 4; }
 };
 template <int NP, int DP, int NW, bool FAST>
 struct SaDkv {
     static constexpr bool DMA = FAST && NP == 1, LATE = NP * DP >= 384;       // LATE: splits at use, nothing staged ahead (registers)
     static constexpr int RT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
-    static constexpr int TILE = NP * RT * DP * 2;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + 2 * RT * 4) + a.G * a.n_dist * 4; }
+    static constexpr bool VL = NP == 1 && DP == 128;           // the wave's values stay in LDS: with them in registers one wave fits a SIMD
+    static constexpr int TILE = NP * RT * DP * 2, VTILE = VL ? NW * 32 * DP * 2 : 0;
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + 2 * RT * 4) + VTILE + a.G * a.row * 4; }
 };
 
-__device__ __forceinline__ void sa_bias_rows(const SaK& a, int h, int heads, float* bt, int nthreads) {
-    for (int i = threadIdx.x; i < heads * a.n_dist; i += nthreads)
-        bt[i] = sa_bias2(a.bias[static_cast<int64_t>(h + i / a.n_dist) * a.n_buckets + max(0, min(a.buckets[i % a.n_dist], a.n_buckets - 1))]);
-}
-
 template <int NP, int DP, int NW, bool FAST>
-__global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq_kernel(const SaK a) {
+__global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_attention_dq_kernel(const SaK a) {
     typedef SaDq<NP, DP, NW, FAST> Cfg;
     constexpr int KT = Cfg::KT, KB = KT / 32, NT = NW * 64, QT = NW * 32, TILE = Cfg::TILE;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint8_t* km0 = reinterpret_cast<uint8_t*>(smem) + Cfg::NBUF * 2 * TILE;
     float* bt = reinterpret_cast<float*>(km0 + Cfg::NBUF * KT);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    float* skew = bt + a.n_dist + wave * SA_SKEW;
-    float* acc = bt + a.n_dist + NW * SA_SKEW + wave * a.n_dist;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    SaLane<NP, DP, KT> ln(lane);
+    float* skew = bt + a.row + wave * SA_SKEW;
+    float* acc0 = bt + a.row + NW * SA_SKEW;
+    float* acc = acc0 + wave * a.n_dist;
+    int* bucket = reinterpret_cast<int*>(acc0 + NW * a.n_dist);
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, within);
@@ -71,6 +70,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
     if (a.bias_part) {
         for (int i = lane; i < SA_SKEW; i += 64) skew[i] = 0.f;
         for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
+        for (int i = threadIdx.x; i < a.n_dist; i += NT) bucket[i] = sa_bucket(a, i);
     }
     float beyond_hi = 0.f, beyond_lo = 0.f;    // ds at distances >= reach / <= -reach (this lane's share)
 
@@ -141,42 +141,51 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
                 __syncthreads();
             }
             if (t + 1 < ntile) fetch(t + 1, buf ^ 1);
-#pragma unroll
+#pragma unroll 1
             for (int kb = 0; kb < KB; ++kb) {
                 const int k0 = t * KT + kb * 32;
                 if (wfirst > wlast || k0 >= sq.lk || (a.causal && k0 > wlast + sq.shift)) continue;      // (whole waves)
+                ln.fresh();
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
                     bf16x8 A[NP];
-                    sa_rows<NP, DP, KT>(kt, kb, s, lane, A);
+                    ln.rows(kt, kb, s, A);
                     S = sa_mma(A, Q[s], S);
-                    sa_rows<NP, DP, KT>(vt, kb, s, lane, A);
+                    ln.rows(vt, kb, s, A);
                     dP = sa_mma(A, dO[s], dP);
                 }
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
-                const bool apart = near_d >= a.reach || far_d <= -a.reach;                               // one bias for the whole block
-                const bool edge = k0 + 32 > sq.lk || (a.causal && near_d < 0) || a.key_mask;
-                const float add = a.n_dist && apart ? bt[sa_entry(near_d >= a.reach ? a.reach : -a.reach, a.reach, a.causal)] : 0.f;
-                float total = 0.f;
+                const SaSpan sp = sa_span(a, near_d, far_d);
+                if (sp.apart) {
+                    const float add = (a.row ? bt[sp.entry] : 0.f) - lse;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at_k = 8 * (i >> 2) + 4 * hi + (i & 3), key = k0 + at_k;
-                    float x = S[i] * a.c + add;
-                    if (a.n_dist && !apart) x += bt[sa_entry(qpos - key, a.reach, a.causal)];
-                    float ds = __builtin_amdgcn_exp2f(x - lse) * (dP[i] - delta);
-                    if (edge) {
-                        bool ok = key < sq.lk && (!a.causal || key <= qpos);
-                        if (a.key_mask) ok = ok && km[kb * 32 + at_k] != 0;
-                        ds = ok ? ds : 0.f;
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + add) * (dP[i] - delta);
+                } else {
+                    const float* be = bt + sa_entry(a, qpos - k0 - 4 * hi - 27);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p = __builtin_amdgcn_exp2f((S[i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)]) - lse);
+                        S[i] = p * (dP[i] - delta);
                     }
-                    S[i] = ds;
-                    total += ds;
+                }
+                if (!a.causal && k0 + 32 > sq.lk) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = k0 + 4 * hi + 8 * (i >> 2) + (i & 3) < sq.lk ? S[i] : 0.f;
+                }
+                if (a.key_mask) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = sa_masked(km + kb * 32 + 4 * hi, i) ? 0.f : S[i];
+                }
+                float total = 0.f;
+                if (a.bias_part && sp.apart) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) total += S[i];
                 }
                 if (a.bias_part) {
                     if (near_d >= a.reach) {
                         beyond_hi += total;
-                    } else if (far_d <= -a.reach) {
+                    } else if (sp.apart) {
                         beyond_lo += total;
                     } else {
 #pragma unroll
@@ -190,7 +199,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
                         const int dist = wfirst + sq.shift - k0 + lane - 31;
                         if (dist >= a.reach) beyond_hi += sum;
                         else if (dist <= -a.reach || (a.causal && dist < 0)) beyond_lo += sum;         // (causal: zeros)
-                        else acc[sa_entry(dist, a.reach, a.causal)] += sum;
+                        else acc[a.causal ? dist : dist + a.reach] += sum;
                     }
                 }
 #pragma unroll
@@ -203,7 +212,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
                         bf16x8 A[NP];
-                        sa_cols<NP, DP, KT>(kt, kb * 2 + ks, db, lane, A);
+                        ln.cols(kt, kb * 2 + ks, db, A);
                         dQ[db] = sa_mma(A, P, dQ[db]);
                     }
                 }
@@ -228,7 +237,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
             if (!a.causal) acc[0] += beyond_lo;
         }
         __syncthreads();
-        float* acc0 = bt + a.n_dist + NW * SA_SKEW;
         for (int i = threadIdx.x; i < a.n_dist; i += NT) {
             float s = acc0[i];
 #pragma unroll
@@ -238,7 +246,8 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP)) void seq_attention_dq
         __syncthreads();
         for (int t = threadIdx.x; t < a.n_buckets; t += NT) {
             float s = 0.f;
-            for (int i = 0; i < a.n_dist; ++i) s += max(0, min(a.buckets[i], a.n_buckets - 1)) == t ? acc0[i] : 0.f;
+#pragma unroll 8
+            for (int i = 0; i < a.n_dist; ++i) s += bucket[i] == t ? acc0[i] : 0.f;
             a.bias_part[(static_cast<int64_t>(h) * a.n_buckets + t) * a.bias_slots + static_cast<int64_t>(b) * a.tiles + tile0] = s;
         }
     }
@@ -255,13 +264,15 @@ __global__ __launch_bounds__(256) void seq_attention_dbias_kernel(const SaK a) {
 }
 
 template <int NP, int DP, int NW, bool FAST>
-__global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_dkv_kernel(const SaK a) {
+__global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_attention_dkv_kernel(const SaK a) {
     typedef SaDkv<NP, DP, NW, FAST> Cfg;
     constexpr int RT = Cfg::RT, RB = RT / 32, NT = NW * 64, KT = NW * 32, TILE = Cfg::TILE;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* rows0 = reinterpret_cast<float*>(smem + Cfg::NBUF * 2 * TILE);      // per buffer: lse of the rows, then delta
+    const sa_lds vt = (sa_lds)smem + Cfg::NBUF * 2 * TILE;
+    float* rows0 = reinterpret_cast<float*>(smem + Cfg::NBUF * 2 * TILE + Cfg::VTILE);      // per buffer: lse of the rows, then delta
     float* tables = rows0 + Cfg::NBUF * 2 * RT;                                // the group's bias rows
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    SaLane<NP, DP, RT> ln(lane);
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, within);
@@ -286,7 +297,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
         const int wlast = min(wfirst + 31, sq.lk - 1);
         SaRows<NP, DP, FAST, Cfg::LATE> K, V;
         K.load(a.k, row * a.k_row + hk * a.k_head, live, a.D, a.vk, lane);
-        V.load(a.v, row * a.v_row + hk * a.v_head, live, a.D, a.vv, lane);
+        if (!Cfg::VL) V.load(a.v, row * a.v_row + hk * a.v_head, live, a.D, a.vv, lane);
         f32x16 dK[DP / 32], dV[DP / 32];
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) { dK[db] = sa_zero16(); dV[db] = sa_zero16(); }
@@ -316,13 +327,22 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
         };
         if (steps > 0) {
             __syncthreads();
+            if constexpr (Cfg::VL) {
+                if constexpr (Cfg::DMA) {
+                    SaDma<DP, KT, NT>::copy(vt, a.v, sq.k0, first, sq.lk, a.v_row, hk * a.v_head, a.D, a.key_mask);
+                } else {
+                    SaStage<NP, DP, KT, NT, FAST> sv;
+                    sv.load(a.v, sq.k0, first, sq.lk, a.v_row, hk * a.v_head, a.D, a.vv, a.key_mask);
+                    sv.store(vt);
+                }
+            }
             if (!Cfg::LATE) fetch(0, 0);
         }
         for (int step = 0; step < steps; ++step) {
             const int q0 = (r_begin + step % n_r) * RT, buf = Cfg::DMA ? step & 1 : 0;
             const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
             float *lse_s = rows0 + buf * 2 * RT, *delta_s = lse_s + RT;
-            const float* bt = tables + (step / n_r) * a.n_dist;
+            const float* bt = tables + (step / n_r) * a.row;
             if (Cfg::LATE) fetch(step, 0);
             if (!Cfg::DMA) {
                 if (step > 0) __syncthreads();
@@ -334,34 +354,39 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
             __syncthreads();
             if (!Cfg::LATE && step + 1 < steps) fetch(step + 1, buf ^ 1);
             if (wfirst > wlast) continue;
-#pragma unroll
+#pragma unroll 1
             for (int rb = 0; rb < RB; ++rb) {
                 const int r0 = q0 + rb * 32, rlast = min(r0 + 31, sq.lq - 1);
                 if (r0 >= sq.lq || (a.causal && rlast + sq.shift < wfirst)) continue;
+                ln.fresh();
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
                     bf16x8 A[NP], B[NP];
-                    sa_rows<NP, DP, RT>(qt, rb, s, lane, A);
+                    ln.rows(qt, rb, s, A);
                     K.get(s, B);
                     S = sa_mma(A, B, S);
-                    sa_rows<NP, DP, RT>(dt, rb, s, lane, A);
-                    V.get(s, B);
+                    ln.rows(dt, rb, s, A);
+                    if constexpr (Cfg::VL) ln.rows(vt + wave * (32 * DP * 2), 0, s, B);
+                    else V.get(s, B);
                     dP = sa_mma(A, B, dP);
                 }
-                const int near_d = r0 + sq.shift - wlast, far_d = rlast + sq.shift - wfirst;
-                const bool apart = near_d >= a.reach || far_d <= -a.reach;
-                const float add = a.n_dist && apart ? bt[sa_entry(near_d >= a.reach ? a.reach : -a.reach, a.reach, a.causal)] : 0.f;
+                // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
+                // behind the last query have lse = +inf, p = 0)
+                const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
+                const float *lr = lse_s + rb * 32 + 4 * hi, *dr = delta_s + rb * 32 + 4 * hi;
+                if (sp.apart) {
+                    const float add = a.row ? bt[sp.entry] : 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at_r = rb * 32 + 8 * (i >> 2) + 4 * hi + (i & 3), dist = q0 + at_r + sq.shift - key;
-                    float x = S[i] * a.c + add;
-                    if (a.n_dist && !apart) x += bt[sa_entry(dist, a.reach, a.causal)];
-                    const bool ok = live && (!a.causal || dist >= 0);
-                    const float p = __builtin_amdgcn_exp2f(x - lse_s[at_r]);
-                    S[i] = ok ? p : 0.f;
-                    dP[i] = ok ? p * (dP[i] - delta_s[at_r]) : 0.f;
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + (add - lr[8 * (i >> 2) + (i & 3)]));
+                } else {
+                    const float* be = bt + sa_entry(a, r0 + 4 * hi + sq.shift - key);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        S[i] = __builtin_amdgcn_exp2f((S[i] * a.c + be[8 * (i >> 2) + (i & 3)]) - lr[8 * (i >> 2) + (i & 3)]);
                 }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
@@ -371,7 +396,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
                     sa_planes_f(f, P);
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
-                        sa_cols<NP, DP, RT>(dt, rb * 2 + ks, db, lane, A);
+                        ln.cols(dt, rb * 2 + ks, db, A);
                         dV[db] = sa_mma(A, P, dV[db]);
                     }
 #pragma unroll
@@ -379,7 +404,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
                     sa_planes_f(f, P);
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
-                        sa_cols<NP, DP, RT>(qt, rb * 2 + ks, db, lane, A);
+                        ln.cols(qt, rb * 2 + ks, db, A);
                         dK[db] = sa_mma(A, P, dK[db]);
                     }
                 }
@@ -392,8 +417,12 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP)) void seq_attention_d
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const int d = db * 32 + 2 * i + 4 * hi;
-                    const float x[4] = {dK[db][i] * a.scale, dK[db][i + 1] * a.scale, dK[db][i + 2] * a.scale, dK[db][i + 3] * a.scale};
-                    const float y[4] = {dV[db][i], dV[db][i + 1], dV[db][i + 2], dV[db][i + 3]};
+                    float x[4], y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[j] = live ? dK[db][i + j] * a.scale : 0.f;
+                        y[j] = live ? dV[db][i + j] : 0.f;
+                    }
                     sa_store4<NP>(a.dk, o, d, a.D, x);
                     sa_store4<NP>(a.dv, o, d, a.D, y);
                 }

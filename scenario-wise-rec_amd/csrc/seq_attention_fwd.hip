@@ -14,14 +14,14 @@
 #include "seq_attention.h"
 
 // waves per SIMD the registers are bounded for (512 / waves each)
-#define SA_WAVES(NP, DP, NW) ((NP) * (DP) >= 384 || ((NP) * (DP) == 192 && (NW) < 4) || ((NP) * (DP) == 128 && (NW) == 1) ? 1 : 2)
+#define SA_WAVES(NP, DP, NW) ((NP) * (DP) >= 384 || ((NP) * (DP) == 192 && (NW) < 4) || ((NP) * (DP) == 128 && (NW) == 1) ? 1 : ((DP) == 32 && ((NP) == 1 || (NW) != 2) ? 3 : 2))
 
 template <int NP, int DP, int NW, bool FAST>
 struct SaFwd {
     static constexpr bool DMA = FAST && NP == 1;               // two buffers filled by LDS-DMA; else one, through registers
     static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr int TILE = NP * KT * DP * 2;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + a.pack * a.n_dist * 4; }
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + a.pack * a.row * 4; }
 };
 
 template <int NP, int DP, int NW, bool FAST>
@@ -31,7 +31,8 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint8_t* km0 = reinterpret_cast<uint8_t*>(smem) + Cfg::NBUF * 2 * TILE;
     float* bt = reinterpret_cast<float*>(km0 + Cfg::NBUF * KT);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    SaLane<NP, DP, KT> ln(lane);
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, within);
@@ -57,14 +58,10 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
     const int ng = a.G / a.pack, g = within % ng;
     const SaSeq sq = sa_seq(a, b);
     const int h0 = hk * a.G + g;
-    for (int i = threadIdx.x; i < a.pack * a.n_dist; i += NT) {
-        const int h = h0 + i / a.n_dist;
-        int bu = a.buckets[i % a.n_dist];
-        if (bu < 0 || bu >= a.n_buckets) {
-            if (a.err_flag) atomicOr(a.err_flag, SWR_FLAG_INDEX_OOR);
-            bu = max(0, min(bu, a.n_buckets - 1));
-        }
-        bt[i] = sa_bias2(a.bias[static_cast<int64_t>(h) * a.n_buckets + bu]);
+    sa_bias_rows(a, h0, a.pack, bt, NT);
+    if (a.n_dist && a.err_flag && unit == 0) {
+        for (int i = threadIdx.x; i < a.n_dist; i += NT)
+            if (a.buckets[i] < 0 || a.buckets[i] >= a.n_buckets) atomicOr(a.err_flag, SWR_FLAG_INDEX_OOR);
     }
 
     const int64_t ncol = static_cast<int64_t>(sq.q_span) * a.pack;
@@ -130,6 +127,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             const int k0 = t * KT;
             if (wfirst > wlast || (a.causal && k0 > wlast + sq.shift)) continue;
 
+            ln.fresh();
             f32x16 S[KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -137,38 +135,36 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
                     bf16x8 A[NP];
-                    sa_rows<NP, DP, KT>(kt, kb, s, lane, A);
+                    ln.rows(kt, kb, s, A);
                     S[kb] = sa_mma(A, Q[s], S[kb]);
                 }
             }
             // scores in the base-2 exponent, with their bias
-            const int near_d = wfirst + sq.shift - (k0 + KT - 1), far_d = wlast + sq.shift - k0;      // range of the wave's distances
-            const float* bh = bt + hsub * a.n_dist;
-            if (a.n_dist && !(near_d >= a.reach || far_d <= -a.reach)) {
+            const float* bh = bt + hsub * a.row;
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = k0 + kb * 32 + 8 * (i >> 2) + 4 * hi + (i & 3);
-                        S[kb][i] = S[kb][i] * a.c + bh[sa_entry(qpos - key, a.reach, a.causal)];
-                    }
-            } else {
-                const float add = a.n_dist ? bh[sa_entry(near_d >= a.reach ? a.reach : -a.reach, a.reach, a.causal)] : 0.f;
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb) {
+                const int kf = k0 + kb * 32;
+                const SaSpan sp = sa_span(a, wfirst + sq.shift - (kf + 31), wlast + sq.shift - kf);
+                if (sp.apart) {
+                    const float add = a.row ? bh[sp.entry] : 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + add;
-            }
-            if (k0 + KT > sq.lk || (a.causal && near_d < 0) || a.key_mask) {
+                } else if (!a.causal || kf <= wlast + sq.shift) {
+                    const float* be = bh + sa_entry(a, qpos - kf - 4 * hi - 27);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                    for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)];
+                } else {                       // a block no query of the wave may see
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at = kb * 32 + 8 * (i >> 2) + 4 * hi + (i & 3), key = k0 + at;
-                        bool ok = key < sq.lk && (!a.causal || key <= qpos);
-                        if (a.key_mask) ok = ok && km[at] != 0;
-                        S[kb][i] = ok ? S[kb][i] : -INFINITY;
-                    }
+                    for (int i = 0; i < 16; ++i) S[kb][i] = -INFINITY;
+                }
+                if (!a.causal && kf + 32 > sq.lk) {                               // (causal: keys behind the last are masked by distance)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[kb][i] = kf + 4 * hi + 8 * (i >> 2) + (i & 3) < sq.lk ? S[kb][i] : -INFINITY;
+                }
+                if (a.key_mask) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[kb][i] = sa_masked(km + kb * 32 + 4 * hi, i) ? -INFINITY : S[kb][i];
+                }
             }
             float mx = m;
 #pragma unroll
@@ -204,7 +200,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
                     bf16x8 A[NP];
-                    sa_cols<NP, DP, KT>(vt, ks, db, lane, A);
+                    ln.cols(vt, ks, db, A);
                     O[db] = sa_mma(A, P, O[db]);
                 }
             }
@@ -302,6 +298,7 @@ SaK sa_args(const swr_seq_attention_args* p) {
     a.Tq = p->Tq; a.Tk = p->Tk; a.B = p->B; a.Hq = p->Hq; a.Hk = p->Hk; a.G = p->Hq / p->Hk; a.D = p->D; a.causal = p->causal != 0;
     a.scale = p->scale; a.c = p->scale * SA_LOG2E;
     a.n_dist = p->n_dist; a.n_buckets = p->n_buckets; a.reach = p->n_dist ? (p->causal ? p->n_dist - 1 : p->n_dist / 2) : 0;
+    a.row = sa_row_entries(p->n_dist, a.reach, a.causal);
     a.q = p->q; a.k = p->k; a.v = p->v;
     a.q_row = p->q_row; a.q_head = p->q_head; a.k_row = p->k_row; a.k_head = p->k_head; a.v_row = p->v_row; a.v_head = p->v_head;
     a.vq = swr_vec8(p->q, p->q_row, p->q_head, p->D, elem);
