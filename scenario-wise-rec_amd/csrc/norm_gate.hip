@@ -32,7 +32,7 @@ struct NgK {
     void *dx, *dy, *dg;                     // contiguous [M, N]
     float* part;                            // [n_wgs][2][N]
     float *dw_post, *dw_pre;
-    int vx, vy, vg, vdz, vdu, vo;
+    int vx, vy, vg, vdz, vdu, vo, vw;
 };
 
 template <int LPR>
@@ -61,12 +61,11 @@ struct NgRow {
     }
 };
 template <int LPR, int MAXC>
-__device__ __forceinline__ void ng_weights(const float* w, int j0, int N, float (&o)[MAXC][8]) {
+__device__ __forceinline__ void ng_weights(const float* w, int j0, int N, int vw, float (&o)[MAXC][8]) {
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
         const int col = (j0 + c * LPR) * 8;
-#pragma unroll
-        for (int v = 0; v < 8; ++v) o[c][v] = (w && col + v < N) ? w[col + v] : 0.f;
+        floats8(load8(w + col, w ? N - col : 0, vw), o[c]);
     }
 }
 template <typename T, int LPR, int MAXC>
@@ -85,8 +84,8 @@ __global__ __launch_bounds__(NG_THREADS) void norm_gate_fwd_kernel(const NgK k) 
     const int j0 = threadIdx.x % LPR, slot = threadIdx.x / LPR;
     const float inv_n = 1.f / static_cast<float>(k.N);
     float wp[MAXC][8], wn[MAXC][8];
-    ng_weights<LPR, MAXC>(k.w_post, j0, k.N, wp);
-    ng_weights<LPR, MAXC>(k.w_pre, j0, k.N, wn);
+    ng_weights<LPR, MAXC>(k.w_post, j0, k.N, k.vw, wp);
+    ng_weights<LPR, MAXC>(k.w_pre, j0, k.N, k.vw, wn);
     int turn = 0;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * SLOTS + slot; r < k.M; r += static_cast<int64_t>(gridDim.x) * SLOTS, turn ^= 1) {
         NgRow<T, MAXC> rx, ry, rg;
@@ -153,8 +152,8 @@ __global__ __launch_bounds__(NG_THREADS) void norm_gate_bwd_kernel(const NgK k) 
     const int j0 = threadIdx.x % LPR, slot = threadIdx.x / LPR;
     const float inv_n = 1.f / static_cast<float>(k.N);
     float wp[MAXC][8], wn[MAXC][8], ap[MAXC][8], an[MAXC][8];
-    ng_weights<LPR, MAXC>(k.w_post, j0, k.N, wp);
-    ng_weights<LPR, MAXC>(k.w_pre, j0, k.N, wn);
+    ng_weights<LPR, MAXC>(k.w_post, j0, k.N, k.vw, wp);
+    ng_weights<LPR, MAXC>(k.w_pre, j0, k.N, k.vw, wn);
 #pragma unroll
     for (int c = 0; c < MAXC; ++c)
 #pragma unroll
@@ -286,8 +285,9 @@ static int ng_lanes(int N) {
 }
 static int ng_wgs(int64_t M, int N, bool backward) {
     const int64_t rows = NG_THREADS / ng_lanes(N), need = std::max<int64_t>(1, swr_ceil_div(M, rows));
-    // backward: two workgroups a CU keep HBM busy (their rows' loads are all in flight) and bound the partials; forward: rows only
-    return static_cast<int>(std::min<int64_t>(need, backward ? NG_MAX_WGS : 8 * NG_MAX_WGS));
+    // two workgroups a CU keep HBM busy in the backward (eight operands' loads in flight) and bound the partials; the forward, with
+    // fewer loads a row, takes four
+    return static_cast<int>(std::min<int64_t>(need, backward ? NG_MAX_WGS : 2 * NG_MAX_WGS));
 }
 static int ng_check(const swr_norm_gate_args* p, bool backward) {
     SWR_REQUIRE(p && p->M >= 0 && p->N >= 1, SWR_ERR_ARG);
@@ -316,6 +316,7 @@ static NgK ng_args(const swr_norm_gate_args* p, bool backward) {
     k.vg = swr_vec8(p->gate, p->ldg, 0, p->N, e);
     k.vdz = swr_vec8(p->dz, p->lddz, 0, p->N, e);
     k.vdu = swr_vec8(p->du, p->lddu, 0, p->N, e);
+    k.vw = std::min(swr_vec8(p->w_post, 0, 0, p->N, 4), swr_vec8(p->w_pre, 0, 0, p->N, 4));
     k.vo = 8;
     void* outs[5] = {p->z, p->u, p->dx, p->dy, p->dgate};
     for (void* o : outs) k.vo = std::min(k.vo, swr_vec8(o, p->N, 0, p->N, e));

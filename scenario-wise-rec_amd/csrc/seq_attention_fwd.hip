@@ -320,6 +320,7 @@ SaK sa_args(const swr_seq_attention_args* p) {
 // 16-byte aligned (one variant for all of them).
 int sa_waves(int64_t columns, const SaK& a, bool fp32) {
     if (!a.fast || (fp32 && a.D > 64)) return 4;
+    if (fp32 && a.D <= 32 && a.pack == 1 && columns <= 256) return 1;
     return columns <= 32 ? 1 : (columns <= 64 ? 2 : 4);
 }
 
@@ -345,7 +346,8 @@ static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     const int64_t wgs = static_cast<int64_t>(a.units) * a.tiles * (a.G / a.pack);
     const int64_t key_tiles = (p->max_k + 63) / 64;
     a.splits = 1;
-    if (wgs > 0 && wgs < 512) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(512 + wgs - 1) / wgs, key_tiles / 2, 64})));
+    const int64_t want = nw == 1 ? 4096 : 512;
+    if (wgs > 0 && wgs < want) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
     a.per_unit = a.tiles * (a.G / a.pack) * a.splits;
 }
 

@@ -2700,9 +2700,15 @@ def block_select(V, domain, D, Hh):
 _SEQ_TYPES = (torch.float32, torch.bfloat16)
 
 
-def _on_device_of(t):
-    """The launches go to the current stream of t's device, whichever device is current."""
-    return torch.cuda.device(t.device)
+def _launch(fn, what, t, *args):
+    """fn(*args, stream): on the current stream of t's device, whichever device is current."""
+    i = t.device.index
+    st = C.c_void_p(torch._C._cuda_getCurrentRawStream(i))
+    if i == torch._C._cuda_getDevice():
+        H.check(fn(*args, st), what)
+    else:
+        with torch.cuda.device(i):
+            H.check(fn(*args, st), what)
 
 
 def _unit_last(t):
@@ -2769,10 +2775,12 @@ class SeqAttention(Function):
         want = any(ctx.needs_input_grad[1:5])
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
         a = _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
-        with _on_device_of(q):
-            nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-            H.check(lib.swr_seq_attention_fwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_seq_attention_fwd")
+        nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _launch(lib.swr_seq_attention_fwd, "swr_seq_attention_fwd", q, C.byref(a), H.ptr(ws), nbytes)
+        if not want:
+            return out
+        ctx.args = a                                               # (addresses of what save_for_backward keeps)
         ctx.save_for_backward(q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         return out
 
@@ -2787,15 +2795,13 @@ class SeqAttention(Function):
         dout = _unit_last(dout if dout.dtype == q.dtype else dout.to(q.dtype))
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[4] else None
-        a = _seq_args(ctx.meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
+        a = ctx.args
         a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        if dbias is not None:
-            a.dbias = dbias.data_ptr()
-        with _on_device_of(q):
-            nbytes = lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            H.check(lib.swr_seq_attention_bwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_seq_attention_bwd")
+        a.dbias = None if dbias is None else dbias.data_ptr()
+        nbytes = lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _launch(lib.swr_seq_attention_bwd, "swr_seq_attention_bwd", q, C.byref(a), H.ptr(ws), nbytes)
         need = ctx.needs_input_grad
         return None, dq if need[1] else None, dk if need[2] else None, dv if need[3] else None, dbias, None, None, None, None, None, None
 
@@ -2896,9 +2902,8 @@ class NormGateResidual(Function):
         ry, rz = stat(w_post), stat(w_pre)
         a = _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz)
         a.z, a.u = (None if z is None else z.data_ptr()), (None if u is None else u.data_ptr())
-        with _on_device_of(x):
-            if M:
-                H.check(lib.swr_norm_gate_fwd(C.byref(a), H.stream()), "swr_norm_gate_fwd")
+        if M:
+            _launch(lib.swr_norm_gate_fwd, "swr_norm_gate_fwd", x, C.byref(a))
         ctx.meta = meta
         ctx.save_for_backward(x, y, gate, w_post, w_pre, ry, rz)
         return z, u
@@ -2927,10 +2932,9 @@ class NormGateResidual(Function):
         for name, t in (("dy", dy), ("dgate", dg), ("dw_post", dwp), ("dw_pre", dwn)):
             if t is not None:
                 setattr(a, name, t.data_ptr())
-        with _on_device_of(x):
-            nbytes = lib.swr_norm_gate_bwd_workspace_bytes(M, N) if dwp is not None or dwn is not None else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            H.check(lib.swr_norm_gate_bwd(C.byref(a), H.ptr(ws), nbytes, H.stream()), "swr_norm_gate_bwd")
+        nbytes = lib.swr_norm_gate_bwd_workspace_bytes(M, N) if dwp is not None or dwn is not None else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _launch(lib.swr_norm_gate_bwd, "swr_norm_gate_bwd", x, C.byref(a), H.ptr(ws), nbytes)
         return None, dx if need[1] else None, dy if need[2] else None, dg if need[3] else None, dwp, dwn
 
 
