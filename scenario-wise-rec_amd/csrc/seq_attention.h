@@ -120,6 +120,20 @@ __device__ __forceinline__ int sa_swz(int row) {
 template <int DP>
 __device__ __forceinline__ int sa_off(int row, int chunk) { return row * (DP * 2) + ((chunk ^ sa_swz<DP>(row)) << 4); }
 
+// x, with what is computed from it kept where it is used: addresses and comparisons hoisted out of the tile loops would fill the
+// vector and scalar registers
+__device__ __forceinline__ int sa_here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// The kernel's arguments read again where they are used: what only the start and the end of a tile need does not sit in scalar
+// registers through its inner loop.
+typedef const __attribute__((address_space(4))) SaK* SaArgs;
+__device__ __forceinline__ SaArgs sa_again() {
+    SaArgs p = (SaArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
 // R rows of a [*, DP] operand moved by NT threads: global -> registers (load), registers -> LDS planes (store).
 // FAST: 16-byte rows and D % 8 == 0 -- every lane loads from a valid address (the last row, the first columns) without a branch and
 // what it should not have read becomes zeros on the way to LDS.  Otherwise 4 or 1 elements at a time under their conditions.
@@ -134,8 +148,7 @@ struct SaStage {
     // rows first .. first + R - 1 of a sequence whose row 0 is `row0`; rows >= limit (limit > first) or masked read as zeros
     __device__ __forceinline__ void load(const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D, int vw,
                                          const uint8_t* mask) {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));          // (addresses are made here, not kept in registers across the tile loop)
+        const int tid = sa_here(threadIdx.x);
         const int chunk = tid % CPR, row = tid / CPR;
         const T* p = static_cast<const T*>(base) + (row0 + first) * stride + head_off;
         keep = 0;
@@ -154,8 +167,7 @@ struct SaStage {
         }
     }
     __device__ __forceinline__ void store(sa_lds dst) const {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));
+        const int tid = sa_here(threadIdx.x);
         const int chunk = tid % CPR, row = tid / CPR;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -185,8 +197,7 @@ struct SaDma {
     static_assert(R * CPR % NT == 0 && NT % CPR == 0, "whole chunks per thread");
     static __device__ __forceinline__ void copy(sa_lds dst, const void* base, int64_t row0, int first, int limit, int64_t stride, int64_t head_off, int D,
                                                 const uint8_t* mask) {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));
+        const int tid = sa_here(threadIdx.x);
         const int slot = tid % CPR, row = tid / CPR;
         const uint16_t* p = static_cast<const uint16_t*>(base) + (row0 + first) * stride + head_off;
         const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)) + (threadIdx.x & ~63u) * 16);
@@ -241,8 +252,9 @@ __device__ __forceinline__ SaRaw<NP> sa_row8(const void* base, int64_t off, int 
 }
 template <int NP, int DP, bool FAST>
 __device__ __forceinline__ void sa_row_frags(const void* base, int64_t off, bool ok, int D, int vw, int lane, bf16x8 (&o)[DP / 16][NP]) {
+    const int col = sa_here(8 * (lane >> 5));
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) sa_planes(sa_row8<NP, FAST>(base, off, 16 * s + 8 * (lane >> 5), ok, D, vw), o[s]);
+    for (int s = 0; s < DP / 16; ++s) sa_planes(sa_row8<NP, FAST>(base, off, 16 * s + col, ok, D, vw), o[s]);
 }
 
 // ... kept as loaded and split at every use where the planes of two operands do not fit the registers (fp32, D > 64: 192 of them)
@@ -261,8 +273,9 @@ template <int NP, int DP, bool FAST>
 struct SaRows<NP, DP, FAST, true> {
     SaRaw<NP> r[DP / 16];
     __device__ __forceinline__ void load(const void* base, int64_t off, bool ok, int D, int vw, int lane) {
+        const int col = sa_here(8 * (lane >> 5));
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) r[s] = sa_row8<NP, FAST>(base, off, 16 * s + 8 * (lane >> 5), ok, D, vw);
+        for (int s = 0; s < DP / 16; ++s) r[s] = sa_row8<NP, FAST>(base, off, 16 * s + col, ok, D, vw);
     }
     __device__ __forceinline__ void get(int s, bf16x8 (&o)[NP]) const {
         float f[8];
@@ -315,7 +328,7 @@ __device__ __forceinline__ int sa_unit(int id, int per_unit, int& within) {
 // comparison.  Blocks wholly beyond the reach take one value.  Without a bias the row is that of a one-entry table of 0, both ways none.
 #define SA_PAD 64
 __host__ __device__ __forceinline__ int sa_row_entries(int n_dist, int reach, int causal) {
-    return (n_dist || causal) ? (causal ? reach : 2 * reach) + 2 * SA_PAD + 1 : 0;
+    return (n_dist || causal) ? ((causal ? reach : 2 * reach) + 2 * SA_PAD + 1 + 3) & ~3 : 0;        // (a multiple of 4: what follows is aligned)
 }
 // bias in the exponent's base-2 unit; a finite value stays finite (a bias of the type's lowest value masks relative to the row's
 // other scores, it does not empty the row)

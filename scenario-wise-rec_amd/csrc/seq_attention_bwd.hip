@@ -7,9 +7,8 @@
 // walks the keys and holds dq (it also makes delta and the bias gradient), a workgroup of key columns walks the queries of all heads
 // of its group and holds dk and dv.  7 products instead of 5, against the fp32 read-modify-write of dq for every key tile.
 //
-// Bias gradient: a 32 x 32 block of ds has 63 distances.  Its wave writes it to LDS so that a distance becomes a row-wise constant
-// column (row k at offset -k), lane t adds up distance t and owns that entry of the wave's per-distance sums.  Blocks wholly beyond
-// the table's reach add their sum to one register.
+// Bias gradient: a 32 x 32 block of ds has 63 distances.  Its wave writes it to LDS skewed, one row per distance, lane t adds up row t
+// and owns that entry of the wave's per-distance sums.  Blocks wholly beyond the table's reach add their sum to one register.
 #include <algorithm>
 
 #include "seq_attention.h"
@@ -22,7 +21,8 @@ unsigned sa_grid(SaK& a);
 // waves per SIMD the registers are bounded for (512 / waves each)
 #define SA_WAVES_DQ(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : 2)
 #define SA_WAVES_DKV(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : ((NP) * (DP) == 32 ? 3 : 2))
-#define SA_SKEW 2048                           // floats of a wave's skewed 32 x 32 block (32 rows of 64)
+#define SA_PITCH 36                            // a wave's skewed 32 x 32 block: one row per distance (63, and one of zeros), 32 keys
+#define SA_SKEW (64 * SA_PITCH)
 
 // dq: DMA and buffers as in the forward; 32 keys a step at DP = 128, so that two workgroups fit a CU's LDS beside the skew blocks
 template <int NP, int DP, int NW, bool FAST>
@@ -30,7 +30,7 @@ struct SaDq {
     static constexpr bool DMA = FAST && NP == 1;
     static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr int TILE = NP * KT * DP * 2;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.row + (a.bias_part ? NW * (SA_SKEW + a.n_dist) + a.n_dist : 0)) * 4; }
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.row + (a.bias_part ? NW * (SA_SKEW + a.n_dist) + a.n_dist + 2 * a.n_buckets : 0)) * 4; }
 };
 template <int NP, int DP, int NW, bool FAST>
 struct SaDkv {
@@ -50,10 +50,10 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
     float* bt = reinterpret_cast<float*>(km0 + Cfg::NBUF * KT);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
     SaLane<NP, DP, KT> ln(lane);
-    float* skew = bt + a.row + wave * SA_SKEW;
+    float* skew = bt + a.row + wave * SA_SKEW;         // (a.row is a multiple of 4)
     float* acc0 = bt + a.row + NW * SA_SKEW;
     float* acc = acc0 + wave * a.n_dist;
-    int* bucket = reinterpret_cast<int*>(acc0 + NW * a.n_dist);
+    int *bucket = reinterpret_cast<int*>(acc0 + NW * a.n_dist), *range = bucket + a.n_dist;
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, within);
@@ -66,12 +66,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
     }
     const int b = unit / a.Hk, hk = unit % a.Hk, g = within % a.G, h = hk * a.G + g, tile0 = a.tiles - 1 - within / a.G;
     const SaSeq sq = sa_seq(a, b);
-    sa_bias_rows(a, h, 1, bt, NT);
-    if (a.bias_part) {
-        for (int i = lane; i < SA_SKEW; i += 64) skew[i] = 0.f;
-        for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
-        for (int i = threadIdx.x; i < a.n_dist; i += NT) bucket[i] = sa_bucket(a, i);
-    }
     float beyond_hi = 0.f, beyond_lo = 0.f;    // ds at distances >= reach / <= -reach (this lane's share)
 
     for (int64_t tile = tile0; tile * QT < sq.q_span; tile += a.tiles) {
@@ -81,29 +75,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
         int kend = a.causal ? min(sq.lk, blast + sq.shift + 1) : sq.lk;
         if (first >= sq.lq || kend < 0) kend = 0;
         const int ntile = (kend + KT - 1) / KT;
-
-        const int64_t row = sq.q0 + (exists ? tok : 0), at = static_cast<int64_t>(h) * a.Tq + row;
-        bf16x8 Q[DP / 16][NP], dO[DP / 16][NP];
-        sa_row_frags<NP, DP, FAST>(a.q, row * a.q_row + static_cast<int64_t>(h) * a.q_head, live, a.D, a.vq, lane, Q);
-        float delta = 0.f;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int col = 16 * s + 8 * hi;
-            const SaRaw<NP> x = sa_row8<NP, FAST>(a.dout, row * a.do_row + static_cast<int64_t>(h) * a.do_head, col, live, a.D, a.vdo);
-            const SaRaw<NP> y = sa_row8<NP, FAST>(a.out, (row * a.Hq + h) * a.D, col, live, a.D, a.vo);
-            float fx[8], fy[8];
-            floats8(x, fx);
-            floats8(y, fy);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
-            sa_planes(x, dO[s]);
-        }
-        delta += __shfl_xor(delta, 32);
-        const float lse = live ? a.lse[at] : INFINITY;
-        if (exists && hi == 0) a.delta[at] = delta;
-        f32x16 dQ[DP / 32];
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) dQ[db] = sa_zero16();
 
         SaStage<NP, DP, KT, NT, FAST> sk, sv;
         uint8_t mk = 1;
@@ -121,10 +92,42 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 mk = key < sq.lk ? a.key_mask[sq.k0 + key] : 0;
             }
         };
-        if (ntile > 0) {
-            __syncthreads();
-            fetch(0, 0);
+        // the first tile's loads go out before anything waits (a tile before this one has been read: barrier first)
+        if (tile != tile0) __syncthreads();
+        if (ntile > 0) fetch(0, 0);
+        const SaArgs n = sa_again();
+        const int64_t row = sq.q0 + (exists ? tok : 0), at = static_cast<int64_t>(h) * n->Tq + row;
+        bf16x8 Q[DP / 16][NP], dO[DP / 16][NP];
+        sa_row_frags<NP, DP, FAST>(n->q, row * n->q_row + static_cast<int64_t>(h) * n->q_head, live, a.D, n->vq, lane, Q);
+        float delta = 0.f;
+        const int hi8 = sa_here(8 * hi);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int col = 16 * s + hi8;
+            const SaRaw<NP> x = sa_row8<NP, FAST>(n->dout, row * n->do_row + static_cast<int64_t>(h) * n->do_head, col, live, a.D, n->vdo);
+            const SaRaw<NP> y = sa_row8<NP, FAST>(n->out, (row * n->Hq + h) * a.D, col, live, a.D, n->vo);
+            float fx[8], fy[8];
+            floats8(x, fx);
+            floats8(y, fy);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
+            sa_planes(x, dO[s]);
         }
+        delta += __shfl_xor(delta, 32);
+        const float lse = live ? n->lse[at] : INFINITY;
+        if (tile == tile0) {
+            sa_bias_rows(a, h, 1, bt, NT);
+            if (a.bias_part) {
+                for (int i = lane; i < SA_SKEW / 4; i += 64) reinterpret_cast<float4*>(skew)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
+                for (int i = threadIdx.x; i < a.n_dist; i += NT) bucket[i] = sa_bucket(a, i);
+            }
+        }
+        if (exists && hi == 0) a.delta[at] = delta;
+        f32x16 dQ[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) dQ[db] = sa_zero16();
+
         for (int t = 0; t < ntile; ++t) {
             const int buf = Cfg::DMA ? t & 1 : 0;
             const sa_lds kt = (sa_lds)smem + buf * 2 * TILE, vt = kt + TILE;
@@ -188,14 +191,18 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                     } else if (sp.apart) {
                         beyond_lo += total;
                     } else {
+                        float* to = skew + (lane & 31) * SA_PITCH + 31 * SA_PITCH - (SA_PITCH - 1) * (4 * hi + 27);      // (lane, key 4 hi + 27)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) skew[(8 * (i >> 2) + 4 * hi + (i & 3)) * 63 + (lane & 31) + 31] = S[i];
+                        for (int i = 0; i < 16; ++i) to[(SA_PITCH - 1) * (27 - 8 * (i >> 2) - (i & 3))] = S[i];
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         float sum = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) sum += skew[k * 64 + lane];
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 x = *reinterpret_cast<const float4*>(skew + lane * SA_PITCH + 4 * k);
+                            sum += (x.x + x.y) + (x.z + x.w);
+                        }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        // column 31 of the skewed block = query wfirst at key k0
+                        // row 31 of the skewed block = the distance of query wfirst to key k0
                         const int dist = wfirst + sq.shift - k0 + lane - 31;
                         if (dist >= a.reach) beyond_hi += sum;
                         else if (dist <= -a.reach || (a.causal && dist < 0)) beyond_lo += sum;         // (causal: zeros)
@@ -219,16 +226,22 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
             }
         }
         if (exists) {
+            const int hi4 = sa_here(4 * hi);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const float x[4] = {dQ[db][i] * a.scale, dQ[db][i + 1] * a.scale, dQ[db][i + 2] * a.scale, dQ[db][i + 3] * a.scale};
-                    sa_store4<NP>(a.dq, (row * a.Hq + h) * a.D, db * 32 + 2 * i + 4 * hi, a.D, x);
+                    sa_store4<NP>(a.dq, (row * a.Hq + h) * a.D, db * 32 + 2 * i + hi4, a.D, x);
                 }
         }
     }
     if (a.bias_part) {
+        if (tile0 * QT >= sq.q_span) {         // nothing of the sequence is this workgroup's
+            for (int t = threadIdx.x; t < a.n_buckets; t += NT)
+                a.bias_part[(static_cast<int64_t>(h) * a.n_buckets + t) * a.bias_slots + static_cast<int64_t>(b) * a.tiles + tile0] = 0.f;
+            return;
+        }
         // entries of the waves -> one per distance -> buckets, all in fixed order
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { beyond_hi += __shfl_xor(beyond_hi, o); beyond_lo += __shfl_xor(beyond_lo, o); }
@@ -236,18 +249,20 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
             acc[a.n_dist - 1] += beyond_hi;
             if (!a.causal) acc[0] += beyond_lo;
         }
+        for (int t = threadIdx.x; t < a.n_buckets; t += NT) { range[2 * t] = a.n_dist; range[2 * t + 1] = 0; }
         __syncthreads();
         for (int i = threadIdx.x; i < a.n_dist; i += NT) {
             float s = acc0[i];
 #pragma unroll
             for (int w = 1; w < NW; ++w) s += acc0[w * a.n_dist + i];
             acc0[i] = s;
+            atomicMin(&range[2 * bucket[i]], i);                   // first entry of a bucket and the one behind its last
+            atomicMax(&range[2 * bucket[i] + 1], i + 1);
         }
         __syncthreads();
         for (int t = threadIdx.x; t < a.n_buckets; t += NT) {
             float s = 0.f;
-#pragma unroll 8
-            for (int i = 0; i < a.n_dist; ++i) s += bucket[i] == t ? acc0[i] : 0.f;
+            for (int i = range[2 * t]; i < range[2 * t + 1]; ++i) s += bucket[i] == t ? acc0[i] : 0.f;
             a.bias_part[(static_cast<int64_t>(h) * a.n_buckets + t) * a.bias_slots + static_cast<int64_t>(b) * a.tiles + tile0] = s;
         }
     }
@@ -288,16 +303,12 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
     }
     const int b = unit / a.Hk, hk = unit % a.Hk;
     const SaSeq sq = sa_seq(a, b);
-    sa_bias_rows(a, hk * a.G, a.G, tables, NT);
     for (int64_t tile = within; tile * KT < sq.k_span; tile += a.tiles) {
         const int first = static_cast<int>(tile * KT), wfirst = first + wave * 32, key = wfirst + (lane & 31);
         const bool exists = key < sq.k_span;
         const int64_t row = sq.k0 + (exists ? key : 0);
         const bool live = key < sq.lk && (!a.key_mask || a.key_mask[row] != 0);
         const int wlast = min(wfirst + 31, sq.lk - 1);
-        SaRows<NP, DP, FAST, Cfg::LATE> K, V;
-        K.load(a.k, row * a.k_row + hk * a.k_head, live, a.D, a.vk, lane);
-        if (!Cfg::VL) V.load(a.v, row * a.v_row + hk * a.v_head, live, a.D, a.vv, lane);
         f32x16 dK[DP / 32], dV[DP / 32];
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) { dK[db] = sa_zero16(); dV[db] = sa_zero16(); }
@@ -325,8 +336,8 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 ld_d = tok < sq.lq ? a.delta[at] : 0.f;
             }
         };
+        if (tile != within) __syncthreads();       // (a tile before this one has been read)
         if (steps > 0) {
-            __syncthreads();
             if constexpr (Cfg::VL) {
                 if constexpr (Cfg::DMA) {
                     SaDma<DP, KT, NT>::copy(vt, a.v, sq.k0, first, sq.lk, a.v_row, hk * a.v_head, a.D, a.key_mask);
@@ -338,6 +349,11 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
             }
             if (!Cfg::LATE) fetch(0, 0);
         }
+        const SaArgs kv = sa_again();
+        SaRows<NP, DP, FAST, Cfg::LATE> K, V;
+        K.load(kv->k, row * kv->k_row + hk * kv->k_head, live, kv->D, kv->vk, lane);
+        if (!Cfg::VL) V.load(kv->v, row * kv->v_row + hk * kv->v_head, live, kv->D, kv->vv, lane);
+        if (tile == within) sa_bias_rows(a, hk * a.G, a.G, tables, NT);
         for (int step = 0; step < steps; ++step) {
             const int q0 = (r_begin + step % n_r) * RT, buf = Cfg::DMA ? step & 1 : 0;
             const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
@@ -412,11 +428,12 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
         }
         if (exists) {
             const int64_t o = (row * a.Hk + hk) * a.D;
+            const int hi4 = sa_here(4 * hi);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    const int d = db * 32 + 2 * i + 4 * hi;
+                    const int d = db * 32 + 2 * i + hi4;
                     float x[4], y[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {

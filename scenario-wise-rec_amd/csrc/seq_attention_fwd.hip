@@ -58,14 +58,14 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
     const int ng = a.G / a.pack, g = within % ng;
     const SaSeq sq = sa_seq(a, b);
     const int h0 = hk * a.G + g;
-    sa_bias_rows(a, h0, a.pack, bt, NT);
     if (a.n_dist && a.err_flag && unit == 0) {
         for (int i = threadIdx.x; i < a.n_dist; i += NT)
             if (a.buckets[i] < 0 || a.buckets[i] >= a.n_buckets) atomicOr(a.err_flag, SWR_FLAG_INDEX_OOR);
     }
 
     const int64_t ncol = static_cast<int64_t>(sq.q_span) * a.pack;
-    for (int64_t tile = a.tiles - 1 - within / ng; tile * QT < ncol; tile += a.tiles) {
+    const int64_t tile0 = a.tiles - 1 - within / ng;
+    for (int64_t tile = tile0; tile * QT < ncol; tile += a.tiles) {
         const int64_t col0 = tile * QT + wave * 32, col = col0 + (lane & 31);
         const int tok = static_cast<int>(min(col, ncol) / a.pack), hsub = static_cast<int>(col % a.pack), h = h0 + hsub;
         const bool exists = col < ncol, live = exists && tok < sq.lq;
@@ -79,13 +79,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
         const int ntile = (kend + KT - 1) / KT;
         const int t0 = static_cast<int>(static_cast<int64_t>(ntile) * split / a.splits);
         const int t1 = static_cast<int>(static_cast<int64_t>(ntile) * (split + 1) / a.splits);
-
-        bf16x8 Q[DP / 16][NP];
-        sa_row_frags<NP, DP, FAST>(a.q, (sq.q0 + (exists ? tok : 0)) * a.q_row + static_cast<int64_t>(h) * a.q_head, live, a.D, a.vq, lane, Q);
-        f32x16 O[DP / 32];
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) O[db] = sa_zero16();
-        float m = -INFINITY, l = 0.f;
 
         SaStage<NP, DP, KT, NT, FAST> sk, sv;
         uint8_t mk = 1;
@@ -103,10 +96,17 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 mk = key < sq.lk ? a.key_mask[sq.k0 + key] : 0;
             }
         };
-        if (t0 < t1) {
-            __syncthreads();                   // (a column tile before this one has been read; the bias table is written)
-            fetch(t0, 0);
-        }
+        // the first tile's loads go out before anything waits (a column tile before this one has been read: barrier first)
+        if (tile != tile0) __syncthreads();
+        if (t0 < t1) fetch(t0, 0);
+        bf16x8 Q[DP / 16][NP];
+        sa_row_frags<NP, DP, FAST>(a.q, (sq.q0 + (exists ? tok : 0)) * a.q_row + static_cast<int64_t>(h) * a.q_head, live, a.D, a.vq, lane, Q);
+        f32x16 O[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) O[db] = sa_zero16();
+        float m = -INFINITY, l = 0.f;
+
+        if (tile == tile0) sa_bias_rows(a, h0, a.pack, bt, NT);
         for (int t = t0; t < t1; ++t) {
             const int buf = Cfg::DMA ? (t - t0) & 1 : 0;
             const sa_lds kt = (sa_lds)smem + buf * 2 * TILE, vt = kt + TILE;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 sa_dma_wait();
                 __syncthreads();
             } else {
-                if (t > t0) __syncthreads();
+                if (t > t0) __syncthreads();           // (the tile's readers are done)
                 sk.store(kt);
                 sv.store(vt);
                 if (a.key_mask && threadIdx.x < KT) km0[threadIdx.x] = mk;
@@ -213,6 +213,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             for (int db = 0; db < DP / 32; ++db) O[db] = sa_zero16();
         }
         if (exists) {
+            const int hi4 = sa_here(4 * hi);
             const int64_t at = static_cast<int64_t>(h) * a.Tq + sq.q0 + tok;
             if (a.splits == 1) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         const float x[4] = {O[db][i] * inv, O[db][i + 1] * inv, O[db][i + 2] * inv, O[db][i + 3] * inv};
-                        sa_store4<NP>(a.out, row, db * 32 + 2 * i + 4 * hi, a.D, x);
+                        sa_store4<NP>(a.out, row, db * 32 + 2 * i + hi4, a.D, x);
                     }
                 if (a.lse && hi == 0) a.lse[at] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
             } else {
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4*>(po + db * 32 + 2 * i + 4 * hi) = make_float4(O[db][i], O[db][i + 1], O[db][i + 2], O[db][i + 3]);
+                        *reinterpret_cast<float4*>(po + db * 32 + 2 * i + hi4) = make_float4(O[db][i], O[db][i + 1], O[db][i + 2], O[db][i + 3]);
             }
         }
     }

@@ -2711,6 +2711,10 @@ def _launch(fn, what, t, *args):
             H.check(fn(*args, st), what)
 
 
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _unit_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -2766,21 +2770,23 @@ class SeqAttention(Function):
     """csrc/seq_attention_fwd.hip / seq_attention_bwd.hip; arguments checked by `seq_attention`."""
 
     @staticmethod
-    def forward(ctx, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
-        ctx.meta = meta
-        if q.numel() == 0 or k.numel() == 0:                       # no query, or no key that any query could see
-            ctx.save_for_backward(q, k, v, bias)
-            return q.new_zeros(q.shape)
+    def launch(want, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
+        """-> out, lse (None unless `want`), the argument block."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        want = any(ctx.needs_input_grad[1:5])
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
         a = _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
         nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         _launch(lib.swr_seq_attention_fwd, "swr_seq_attention_fwd", q, C.byref(a), H.ptr(ws), nbytes)
-        if not want:
-            return out
-        ctx.args = a                                               # (addresses of what save_for_backward keeps)
+        return out, lse, a
+
+    @staticmethod
+    def forward(ctx, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
+        if q.numel() == 0 or k.numel() == 0:                       # no query, or no key that any query could see
+            ctx.save_for_backward(q, k, v, bias)
+            return q.new_zeros(q.shape)
+        out, lse, ctx.args = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+        # (ctx.args: addresses of what is kept here)
         ctx.save_for_backward(q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         return out
 
@@ -2871,7 +2877,10 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
     meta = {"causal": bool(causal), "scale": float(D ** -0.5 if scale is None else scale),
             "max_q": q.shape[0] if max_q is None else min(int(max_q), q.shape[0]),
             "max_k": k.shape[0] if max_k is None else min(int(max_k), k.shape[0])}
-    return SeqAttention.apply(meta, _unit_last(q), _unit_last(k), _unit_last(v), bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+    args = (meta, _unit_last(q), _unit_last(k), _unit_last(v), bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+    if not _needs_grad(q, k, v, bias) and q.numel() and k.numel():
+        return SeqAttention.launch(False, *args)[0]               # (serving: without the tape's bookkeeping)
+    return SeqAttention.apply(*args)
 
 
 def _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz):
@@ -2892,18 +2901,23 @@ class NormGateResidual(Function):
     """csrc/norm_gate.hip; arguments checked by `norm_gate_residual`.  Returns (z or None, u or None)."""
 
     @staticmethod
-    def forward(ctx, meta, x, y, gate, w_post, w_pre):
-        ctx.set_materialize_grads(False)
+    def launch(want, meta, x, y, gate, w_post, w_pre):
+        """-> z, u, and the rows' statistics (None unless `want`)."""
         dev, M = x.device, x.shape[0]
         z = torch.empty(x.shape, dtype=x.dtype, device=dev) if y is not None else None
         u = torch.empty(x.shape, dtype=x.dtype, device=dev) if w_pre is not None else None
-        want = any(ctx.needs_input_grad)
-        stat = lambda w: torch.empty(M, dtype=torch.float32, device=dev) if want and w is not None else None
-        ry, rz = stat(w_post), stat(w_pre)
-        a = _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz)
-        a.z, a.u = (None if z is None else z.data_ptr()), (None if u is None else u.data_ptr())
+        ry = torch.empty(M, dtype=torch.float32, device=dev) if want and w_post is not None else None
+        rz = torch.empty(M, dtype=torch.float32, device=dev) if want and w_pre is not None else None
         if M:
+            a = _norm_gate_args(meta, x, y, gate, w_post, w_pre, ry, rz)
+            a.z, a.u = (None if z is None else z.data_ptr()), (None if u is None else u.data_ptr())
             _launch(lib.swr_norm_gate_fwd, "swr_norm_gate_fwd", x, C.byref(a))
+        return z, u, ry, rz
+
+    @staticmethod
+    def forward(ctx, meta, x, y, gate, w_post, w_pre):
+        ctx.set_materialize_grads(False)
+        z, u, ry, rz = NormGateResidual.launch(True, meta, x, y, gate, w_post, w_pre)
         ctx.meta = meta
         ctx.save_for_backward(x, y, gate, w_post, w_pre, ry, rz)
         return z, u
@@ -2961,6 +2975,6 @@ def norm_gate_residual(x, y=None, gate=None, w_post=None, w_pre=None, scale=1.0,
             raise ValueError(f"norm_gate_residual: {name} must be float32 [{x.shape[1]}] on {x.device}, got {t.dtype} {tuple(t.shape)}")
     flat = lambda t: None if t is None else _unit_last(t)
     meta = {"scale": float(scale), "eps": float(eps)}
-    z, u = NormGateResidual.apply(meta, flat(x), flat(y), flat(gate), None if w_post is None else w_post.contiguous(),
-                                  None if w_pre is None else w_pre.contiguous())
+    args = (meta, flat(x), flat(y), flat(gate), None if w_post is None else w_post.contiguous(), None if w_pre is None else w_pre.contiguous())
+    z, u = NormGateResidual.apply(*args) if _needs_grad(x, y, gate, w_post, w_pre) else NormGateResidual.launch(False, *args)[:2]
     return u if y is None else (z if w_pre is None else (z, u))
