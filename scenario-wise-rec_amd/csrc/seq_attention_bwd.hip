@@ -56,7 +56,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
     int *bucket = reinterpret_cast<int*>(acc0 + NW * a.n_dist), *range = bucket + a.n_dist;
 
     int within;
-    const int unit = sa_unit(blockIdx.x, a.per_unit, within);
+    const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
     if (unit > a.units) return;
     if (unit == a.units) {                     // rows of no sequence
         const int64_t end0 = sa_clamp(a.cu_q[0], 0, a.Tq), beg1 = sa_clamp(a.cu_q[a.B], end0, a.Tq), row = static_cast<int64_t>(a.Hq) * a.D;
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
     SaLane<NP, DP, RT> ln(lane);
 
     int within;
-    const int unit = sa_unit(blockIdx.x, a.per_unit, within);
+    const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
     if (unit > a.units) return;
     if (unit == a.units) {                     // rows of no sequence
         const int64_t end0 = sa_clamp(a.cu_k[0], 0, a.Tk), beg1 = sa_clamp(a.cu_k[a.B], end0, a.Tk), row = static_cast<int64_t>(a.Hk) * a.D;

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
     SaLane<NP, DP, KT> ln(lane);
 
     int within;
-    const int unit = sa_unit(blockIdx.x, a.per_unit, within);
+    const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
     if (unit > a.units) return;
     if (unit == a.units) {                     // rows of no sequence
         const int64_t end0 = sa_clamp(a.cu_q[0], 0, a.Tq), beg1 = sa_clamp(a.cu_q[a.B], end0, a.Tq);
@@ -327,7 +327,9 @@ int sa_waves(int64_t columns, const SaK& a, bool fp32) {
 
 // workgroups of a launch (the rows of no sequence are one more unit), or 0 when they do not fit a grid
 unsigned sa_grid(SaK& a) {
-    const int64_t slots = (static_cast<int64_t>(a.units) + 1 + 7) / 8;
+    const int64_t each = (static_cast<int64_t>(a.units) + 1 + 7) / 8;               // units per XCD
+    if (a.together <= 0 || a.together > each) a.together = static_cast<int>(each);
+    const int64_t slots = (each + a.together - 1) / a.together * a.together;
     const int64_t max_per_unit = ((1ll << 30) / 8) / slots;
     const int64_t rest = static_cast<int64_t>(a.per_unit / a.tiles);
     if (rest > max_per_unit) return 0;
@@ -350,6 +352,7 @@ static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     const int64_t want = nw == 1 ? 4096 : 512;
     if (wgs > 0 && wgs < want) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
     a.per_unit = a.tiles * (a.G / a.pack) * a.splits;
+    a.together = 1;
 }
 
 extern "C" size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_args* p) {
