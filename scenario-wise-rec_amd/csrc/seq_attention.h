@@ -191,6 +191,9 @@ __device__ __forceinline__ void sa_dma16(uint32_t lds_addr, const void* src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr), "v"(src) : "memory", "m0");
 }
 __device__ __forceinline__ void sa_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void sa_dma16(uint32_t lds_addr, uint32_t offset, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(offset), "s"(base) : "memory", "m0");
+}
 template <int DP, int R, int NT>
 struct SaDma {
     static constexpr int CPR = DP / 8, N = R * CPR / NT, STEP = NT / CPR;
@@ -201,6 +204,14 @@ struct SaDma {
         const int slot = tid % CPR, row = tid / CPR;
         const uint16_t* p = static_cast<const uint16_t*>(base) + (row0 + first) * stride + head_off;
         const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)) + (threadIdx.x & ~63u) * 16);
+        if (D == DP && first + R <= limit && !mask) {              // every piece counts: one offset per lane, the rest is scalar
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int same = STEP % 16 == 0 ? row : row + i * STEP;        // (rows 16 apart have the same swizzle)
+                sa_dma16(at + i * NT * 16, 2 * (static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) + (slot ^ sa_swz<DP>(same)) * 8), p + i * STEP * stride);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int rr = row + i * STEP, col = (slot ^ sa_swz<DP>(rr)) * 8;

@@ -14,12 +14,14 @@
 #include "seq_attention.h"
 
 // waves per SIMD the registers are bounded for (512 / waves each)
-#define SA_WAVES(NP, DP, NW) ((NP) * (DP) >= 384 || ((NP) * (DP) == 192 && (NW) < 4) || ((NP) * (DP) == 128 && (NW) == 1) ? 1 : ((DP) == 32 && ((NP) == 1 || (NW) != 2) ? 3 : 2))
+#define SA_WAVES(NP, DP, NW) ((NP) * (DP) >= 384 || ((NP) * (DP) == 192 && (NW) < 4) || ((NP) * (DP) == 128 && (NW) == 1) ? 1 : (((DP) == 32 && (NW) == 1) || (NP) * (DP) == 64 ? 3 : 2))
 
 template <int NP, int DP, int NW, bool FAST>
 struct SaFwd {
     static constexpr bool DMA = FAST && NP == 1;               // two buffers filled by LDS-DMA; else one, through registers
-    static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
+    // keys per tile: 64 where two waves a SIMD have the registers for it, 32 where that makes room for a third (bf16, D <= 64: 0.896 /
+    // 0.880 ms for the packed training step) or where one wave stages alone (prompts of 128 a head, 64 against 32: 2.49 / 2.57 ms)
+    static constexpr int KT = (NW == 1 || (DP == 128 && !(DMA && NW == 4)) || (NP == 1 && DP == 64)) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr int TILE = NP * KT * DP * 2;
     static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + a.pack * a.row * 4; }
 };
@@ -139,57 +141,70 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                     S[kb] = sa_mma(A, Q[s], S[kb]);
                 }
             }
-            // scores in the base-2 exponent, with their bias
+            // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
+            // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
             const float* bh = bt + hsub * a.row;
+            float mul[KB], add[KB], mx = -INFINITY;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const int kf = k0 + kb * 32;
                 const SaSpan sp = sa_span(a, wfirst + sq.shift - (kf + 31), wlast + sq.shift - kf);
-                if (sp.apart) {
-                    const float add = a.row ? bh[sp.entry] : 0.f;
+                const bool cut = !a.causal && kf + 32 > sq.lk;                    // (causal: keys behind the last are masked by distance)
+                mul[kb] = a.c;
+                add[kb] = sp.apart && a.row ? bh[sp.entry] : 0.f;
+                if (!sp.apart || cut || a.key_mask || a.c < 0.f) {
+                    if (sp.apart) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + add;
-                } else if (!a.causal || kf <= wlast + sq.shift) {
-                    const float* be = bh + sa_entry(a, qpos - kf - 4 * hi - 27);
+                        for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + add[kb];
+                    } else if (!a.causal || kf <= wlast + sq.shift) {
+                        const float* be = bh + sa_entry(a, qpos - kf - 4 * hi - 27);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)];
-                } else {                       // a block no query of the wave may see
+                        for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)];
+                    } else {                   // a block no query of the wave may see
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[kb][i] = -INFINITY;
+                        for (int i = 0; i < 16; ++i) S[kb][i] = -INFINITY;
+                    }
+                    mul[kb] = 1.f;
+                    add[kb] = 0.f;
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) S[kb][i] = kf + 4 * hi + 8 * (i >> 2) + (i & 3) < sq.lk ? S[kb][i] : -INFINITY;
+                    }
+                    if (a.key_mask) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) S[kb][i] = sa_masked(km + kb * 32 + 4 * hi, i) ? -INFINITY : S[kb][i];
+                    }
                 }
-                if (!a.causal && kf + 32 > sq.lk) {                               // (causal: keys behind the last are masked by distance)
+                float top = S[kb][0];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[kb][i] = kf + 4 * hi + 8 * (i >> 2) + (i & 3) < sq.lk ? S[kb][i] : -INFINITY;
-                }
-                if (a.key_mask) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[kb][i] = sa_masked(km + kb * 32 + 4 * hi, i) ? -INFINITY : S[kb][i];
-                }
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, S[kb][i]);
+                mx = fmaxf(mx, top * mul[kb] + add[kb]);
             }
-            float mx = m;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[kb][i]);
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float ms = mx == -INFINITY ? 0.f : mx;
-            const float corr = __builtin_amdgcn_exp2f(m - ms);
-            float sum = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    S[kb][i] = __builtin_amdgcn_exp2f(S[kb][i] - ms);
-                    sum += S[kb][i];
-                }
-            l = l * corr + sum;
-            if (__any(mx != m)) {
+            // The reference exponent m follows the maximum only in steps of 2^8 (p and l stay below 2^8 times the row's length): O is
+            // rescaled in the first tile and hardly ever again, not whenever one of 32 rows finds a new maximum.
+            if (__any(mx > m + 8.f)) {
+                const float up = mx > m + 8.f ? mx : m;
+                const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= corr;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) O[db][i] *= corr;
             }
-            m = mx;
+            const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const float sh = add[kb] - ms;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    S[kb][i] = __builtin_amdgcn_exp2f(S[kb][i] * mul[kb] + sh);
+                    sum += S[kb][i];
+                }
+                l += sum;
+            }
 #pragma unroll
             for (int ks = 0; ks < KT / 16; ++ks) {
                 float pf[8];
