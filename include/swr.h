@@ -831,6 +831,8 @@ typedef struct {
     const void* v; int64_t v_row, v_head;
     void* out;
     float* lse;                        /* [Hq, Tq] log2 of the softmax sums, +inf for an empty row; NULL in a forward without a backward */
+    float* out32;                      /* SWR_BF16 with lse: out before its rounding, [Tq, Hq, D], kept for the backward (its row products
+                                          do . o have to agree with the score gradients' fp32 sums); SWR_F32: not used */
     const int32_t* cu_q; const int32_t* cu_k; const int32_t* q_len; const int32_t* k_len;
     const uint8_t* key_mask;           /* [Tk], nullable */
     const float* bias;                 /* [Hq, n_buckets] */

@@ -32,7 +32,7 @@ struct SaK {
     int vq, vk, vv, vo, vdo;               // elements per load of q, k, v, out, dout rows: 8, 4 or 1
     bool fast;                             // all of them 8, row strides below 2^23 elements (64 rows within 32-bit byte offsets)
     const void *q, *k, *v; int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-    void* out; float* lse;
+    void* out; float* lse; float* out32;
     const int32_t *cu_q, *cu_k, *q_len, *k_len;
     const uint8_t* key_mask;
     const float* bias; const int32_t* buckets;
@@ -92,6 +92,20 @@ __device__ __forceinline__ void sa_planes_f(const float* f, bf16x8 (&o)[1]) {
     for (int j = 0; j < 8; j += 2) CVT_PAIR(f[j], f[j + 1], o[0], j);
 }
 
+// ... and to 2^-17 in two planes: the probabilities of a training forward on bf16 tensors
+__device__ __forceinline__ void sa_planes_f(const float* f, bf16x8 (&o)[2]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        CVT_PAIR(f[j], f[j + 1], o[0], j);
+        const float r0 = f[j] - static_cast<float>(o[0][j]), r1 = f[j + 1] - static_cast<float>(o[0][j + 1]);
+        CVT_PAIR(r0, r1, o[1], j);
+    }
+}
+
+__device__ __forceinline__ f32x16 sa_mma(const bf16x8 (&a)[1], const bf16x8 (&b)[2], f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16 sa_mma(const bf16x8 (&a)[1], const bf16x8 (&b)[1], f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
 }

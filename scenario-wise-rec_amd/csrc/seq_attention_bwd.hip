@@ -105,7 +105,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
         for (int s = 0; s < DP / 16; ++s) {
             const int col = 16 * s + hi8;
             const SaRaw<NP> x = sa_row8<NP, FAST>(n->dout, row * n->do_row + static_cast<int64_t>(h) * n->do_head, col, live, a.D, n->vdo);
-            const SaRaw<NP> y = sa_row8<NP, FAST>(n->out, (row * n->Hq + h) * a.D, col, live, a.D, n->vo);
+            const SaRaw<3> y = sa_row8<3, FAST>(n->out32, (row * n->Hq + h) * a.D, col, live, a.D, n->vo);
             float fx[8], fy[8];
             floats8(x, fx);
             floats8(y, fy);

@@ -26,7 +26,10 @@ struct SaFwd {
     static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + a.pack * a.row * 4; }
 };
 
-template <int NP, int DP, int NW, bool FAST>
+// TRAIN (bf16): the probabilities enter the second product in two planes and the unrounded rows are kept.  The backward's delta = do . o
+// has to agree with its fp32 sums of p (do . v): with o from probabilities rounded to 2^-9 the bias gradient, whose terms nearly cancel
+// in every row, was off by 2.8e-3 of its norm.
+template <int NP, int DP, int NW, bool FAST, bool TRAIN>
 __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_fwd_kernel(const SaK a) {
     typedef SaFwd<NP, DP, NW, FAST> Cfg;
     constexpr int KT = Cfg::KT, KB = KT / 32, NT = NW * 64, QT = NW * 32, TILE = Cfg::TILE;
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 float pf[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pf[j] = S[ks >> 1][8 * (ks & 1) + j];
-                bf16x8 P[NP];
+                bf16x8 P[TRAIN ? 2 : NP];
                 sa_planes_f(pf, P);
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
@@ -239,6 +242,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                     for (int i = 0; i < 16; i += 4) {
                         const float x[4] = {O[db][i] * inv, O[db][i + 1] * inv, O[db][i + 2] * inv, O[db][i + 3] * inv};
                         sa_store4<NP>(a.out, row, db * 32 + 2 * i + hi4, a.D, x);
+                        if (TRAIN) sa_store4<3>(a.out32, row, db * 32 + 2 * i + hi4, a.D, x);
                     }
                 if (a.lse && hi == 0) a.lse[at] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
             } else {
@@ -280,6 +284,7 @@ __global__ __launch_bounds__(256) void seq_attention_join_kernel(const SaK a) {
     const int64_t h = at / a.Tq, t = at % a.Tq;
     const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     sa_store4<NP>(a.out, (t * a.Hq + h) * a.D, 4 * j, a.D, x);
+    if (NP == 1 && a.out32) sa_store4<3>(a.out32, (t * a.Hq + h) * a.D, 4 * j, a.D, x);
     if (a.lse && j == 0) a.lse[at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
@@ -300,9 +305,9 @@ int sa_check(const swr_seq_attention_args* p, bool backward) {
         SWR_REQUIRE(p->n_dist <= SWR_SEQ_MAX_DIST && p->n_buckets <= SWR_SEQ_MAX_BUCKETS && (p->causal || p->n_dist % 2 == 1), SWR_ERR_UNSUPPORTED);
         SWR_REQUIRE(static_cast<int64_t>(p->n_dist) * (p->Hq / p->Hk) <= SWR_SEQ_MAX_TABLE, SWR_ERR_UNSUPPORTED);
     }
-    SWR_REQUIRE((reinterpret_cast<uintptr_t>(p->out) & 15) == 0, SWR_ERR_ALIGN);
+    SWR_REQUIRE(((reinterpret_cast<uintptr_t>(p->out) | reinterpret_cast<uintptr_t>(p->out32)) & 15) == 0, SWR_ERR_ALIGN);
     if (backward) {
-        SWR_REQUIRE(p->lse && p->dout && p->dq && p->dk && p->dv, SWR_ERR_ARG);
+        SWR_REQUIRE(p->lse && (p->out32 || p->dtype == SWR_F32) && p->dout && p->dq && p->dk && p->dv, SWR_ERR_ARG);
         SWR_REQUIRE(((reinterpret_cast<uintptr_t>(p->dq) | reinterpret_cast<uintptr_t>(p->dk) | reinterpret_cast<uintptr_t>(p->dv)) & 15) == 0, SWR_ERR_ALIGN);
     }
     return SWR_OK;
@@ -320,10 +325,11 @@ SaK sa_args(const swr_seq_attention_args* p) {
     a.vq = swr_vec8(p->q, p->q_row, p->q_head, p->D, elem);
     a.vk = swr_vec8(p->k, p->k_row, p->k_head, p->D, elem);
     a.vv = swr_vec8(p->v, p->v_row, p->v_head, p->D, elem);
-    a.vo = swr_vec8(p->out, static_cast<int64_t>(p->Hq) * p->D, p->D, p->D, elem);
+    a.vo = swr_vec8(p->out, static_cast<int64_t>(p->Hq) * p->D, p->D, p->D, 4);
     a.vdo = swr_vec8(p->dout, p->do_row, p->do_head, p->D, elem);
     const int64_t far = 1ll << 23;
     a.fast = a.vq == 8 && a.vk == 8 && a.vv == 8 && (!p->dout || a.vdo == 8) && p->q_row < far && p->k_row < far && p->v_row < far && p->do_row < far;
+    a.out32 = p->dtype == SWR_F32 ? static_cast<float*>(p->out) : p->out32;
     a.out = p->out; a.lse = p->lse; a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.q_len = p->q_len; a.k_len = p->k_len; a.key_mask = p->key_mask;
     a.bias = p->bias; a.buckets = p->buckets; a.dout = p->dout; a.do_row = p->do_row; a.do_head = p->do_head;
     a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.dbias = p->dbias; a.err_flag = p->err_flag;
@@ -379,29 +385,30 @@ extern "C" size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_
     return a.splits == 1 ? 0 : static_cast<size_t>(a.splits) * a.Hq * a.Tq * (2 + dp) * sizeof(float);
 }
 
-template <int NP, int DP, int NW, bool FAST>
+template <int NP, int DP, int NW, bool FAST, bool TRAIN>
 static int sa_fwd_launch(SaK& a, hipStream_t st) {
     const int lds = SaFwd<NP, DP, NW, FAST>::lds(a);
-    const void* fn = reinterpret_cast<const void*>(seq_attention_fwd_kernel<NP, DP, NW, FAST>);
+    const void* fn = reinterpret_cast<const void*>(seq_attention_fwd_kernel<NP, DP, NW, FAST, TRAIN>);
     if (lds > 64 * 1024 && !swr_raise_lds(fn, 160 * 1024)) return SWR_ERR_LAUNCH;
     const unsigned grid = sa_grid(a);
     SWR_REQUIRE(grid, SWR_ERR_UNSUPPORTED);
-    hipLaunchKernelGGL((seq_attention_fwd_kernel<NP, DP, NW, FAST>), dim3(grid), dim3(NW * 64), lds, st, a);
+    hipLaunchKernelGGL((seq_attention_fwd_kernel<NP, DP, NW, FAST, TRAIN>), dim3(grid), dim3(NW * 64), lds, st, a);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.Hq) * a.Tq;
         hipLaunchKernelGGL((seq_attention_join_kernel<NP, DP>), dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, a);
     }
     return swr_launch_status();
 }
-template <int NP, int DP>
+template <int NP, int DP, bool TRAIN>
 static int sa_fwd_nw(SaK& a, int nw, hipStream_t st) {
-    if (!a.fast) return sa_fwd_launch<NP, DP, 4, false>(a, st);
-    if constexpr (NP * DP >= 384) return sa_fwd_launch<NP, DP, 4, true>(a, st);
-    else return nw == 1 ? sa_fwd_launch<NP, DP, 1, true>(a, st) : (nw == 2 ? sa_fwd_launch<NP, DP, 2, true>(a, st) : sa_fwd_launch<NP, DP, 4, true>(a, st));
+    if (!a.fast) return sa_fwd_launch<NP, DP, 4, false, TRAIN>(a, st);
+    if constexpr (NP * DP >= 384) return sa_fwd_launch<NP, DP, 4, true, TRAIN>(a, st);
+    else return nw == 1 ? sa_fwd_launch<NP, DP, 1, true, TRAIN>(a, st)
+                        : (nw == 2 ? sa_fwd_launch<NP, DP, 2, true, TRAIN>(a, st) : sa_fwd_launch<NP, DP, 4, true, TRAIN>(a, st));
 }
-template <int NP>
+template <int NP, bool TRAIN>
 static int sa_fwd_dp(SaK& a, int nw, hipStream_t st) {
-    return a.D <= 32 ? sa_fwd_nw<NP, 32>(a, nw, st) : (a.D <= 64 ? sa_fwd_nw<NP, 64>(a, nw, st) : sa_fwd_nw<NP, 128>(a, nw, st));
+    return a.D <= 32 ? sa_fwd_nw<NP, 32, TRAIN>(a, nw, st) : (a.D <= 64 ? sa_fwd_nw<NP, 64, TRAIN>(a, nw, st) : sa_fwd_nw<NP, 128, TRAIN>(a, nw, st));
 }
 
 extern "C" int swr_seq_attention_fwd(const swr_seq_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -419,5 +426,6 @@ extern "C" int swr_seq_attention_fwd(const swr_seq_attention_args* p, void* work
         a.part = static_cast<float*>(workspace);
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    return p->dtype == SWR_F32 ? sa_fwd_dp<3>(a, nw, st) : sa_fwd_dp<1>(a, nw, st);
+    if (p->dtype == SWR_F32) return sa_fwd_dp<3, false>(a, nw, st);
+    return a.out32 ? sa_fwd_dp<1, true>(a, nw, st) : sa_fwd_dp<1, false>(a, nw, st);
 }

@@ -161,7 +161,7 @@ class SeqAttentionArgs(C.Structure):
                 ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
                 ("k", C.c_void_p), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v", C.c_void_p), ("v_row", C.c_int64), ("v_head", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
-                ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_len", C.c_void_p), ("k_len", C.c_void_p),
+                ("out32", C.c_void_p), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_len", C.c_void_p), ("k_len", C.c_void_p),
                 ("key_mask", C.c_void_p), ("bias", C.c_void_p), ("buckets", C.c_void_p),
                 ("dout", C.c_void_p), ("do_row", C.c_int64), ("do_head", C.c_int64),
                 ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dbias", C.c_void_p), ("err_flag", C.c_void_p)]

@@ -2744,7 +2744,7 @@ def seq_buckets(n_buckets, max_distance, causal=True, device="cuda"):
     return torch.tensor(table, dtype=torch.int32, device=device)
 
 
-def _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets):
+def _seq_args(meta, q, k, v, out, lse, out32, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets):
     a = H.SeqAttentionArgs()
     a.Tq, a.Tk, a.B, a.Hq, a.Hk, a.D = q.shape[0], k.shape[0], cu_q.numel() - 1, q.shape[1], k.shape[1], q.shape[2]
     a.dtype, a.causal, a.max_q, a.max_k, a.scale = H.dtype_code(q), int(meta["causal"]), meta["max_q"], meta["max_k"], meta["scale"]
@@ -2754,6 +2754,8 @@ def _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias,
     a.out, a.cu_q, a.cu_k = out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr()
     if lse is not None:
         a.lse = lse.data_ptr()
+    if out32 is not None:
+        a.out32 = out32.data_ptr()
     if q_len is not None:
         a.q_len = q_len.data_ptr()
     if k_len is not None:
@@ -2771,23 +2773,24 @@ class SeqAttention(Function):
 
     @staticmethod
     def launch(want, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
-        """-> out, lse (None unless `want`), the argument block."""
+        """-> out, what the backward needs besides (None unless `want`), the argument block."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
-        a = _seq_args(meta, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
+        out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want and q.dtype != torch.float32 else None
+        a = _seq_args(meta, q, k, v, out, lse, out32, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
         nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         _launch(lib.swr_seq_attention_fwd, "swr_seq_attention_fwd", q, C.byref(a), H.ptr(ws), nbytes)
-        return out, lse, a
+        return out, lse, out if out32 is None else out32, a
 
     @staticmethod
     def forward(ctx, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
         if q.numel() == 0 or k.numel() == 0:                       # no query, or no key that any query could see
             ctx.save_for_backward(q, k, v, bias)
             return q.new_zeros(q.shape)
-        out, lse, ctx.args = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+        out, lse, out32, ctx.args = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         # (ctx.args: addresses of what is kept here)
-        ctx.save_for_backward(q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+        ctx.save_for_backward(q, k, v, bias, out32, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         return out
 
     @staticmethod
@@ -2796,7 +2799,7 @@ class SeqAttention(Function):
         if len(ctx.saved_tensors) == 4:
             return (None,) + tuple(torch.zeros_like(t) if t is not None and n else None
                                    for t, n in zip(ctx.saved_tensors, ctx.needs_input_grad[1:5])) + (None,) * 6
-        q, k, v, bias, out, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets = ctx.saved_tensors
+        q, k, v, bias, _out32, _lse, *_index = ctx.saved_tensors      # (all of it is in ctx.args by address)
         dev = q.device
         dout = _unit_last(dout if dout.dtype == q.dtype else dout.to(q.dtype))
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))

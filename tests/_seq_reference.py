@@ -12,11 +12,15 @@ def f(n):
     return (6 * n / 16 + 24) * 2.0 ** -24
 
 
-def attention(q, k, v, dout, qs, ks, q0, k0, causal, scale=None, bias=None, buckets=None, key_mask=None):
-    """Lists of lengths and first rows per sequence.  -> {name: (value, allowed error)} for out, dq, dk, dv, dbias, in 64 bits."""
+def attention(q, k, v, dout, qs, ks, q0, k0, causal, scale=None, bias=None, buckets=None, key_mask=None, train=True):
+    """Lists of lengths and first rows per sequence.  -> {name: (value, allowed error)} for out, dq, dk, dv, dbias, in 64 bits.
+    bf16: p enters its product rounded to bf16, in a training forward in two bf16 terms (2^-16 of p at most remains); the backward's
+    delta starts from the unrounded rows of that forward, and the bias gradient sums fp32 values that were never rounded further."""
     dt, dev = q.dtype, q.device
-    u = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -24
-    r = u if dt == torch.bfloat16 else f(16)                      # rounding of p and ds before they are multiplied
+    bf16 = dt == torch.bfloat16
+    u = 2.0 ** -8 if bf16 else 2.0 ** -24
+    r = u if bf16 else f(16)                                      # rounding of p and ds before they are multiplied, backward
+    rf = (2.0 ** -16 if train else u) if bf16 else r              # ... of p, forward
     H, Hk, D = q.shape[1], k.shape[1], q.shape[2]
     G = H // Hk
     scale = D ** -0.5 if scale is None else scale
@@ -52,14 +56,13 @@ def attention(q, k, v, dout, qs, ks, q0, k0, causal, scale=None, bias=None, buck
             row = es.max(1, keepdim=True).values if lk else top
             ep = (es + row + 2.0 ** -20) * p                      # ... of p: numerator, sum of the row, exp2 and division
             o = p @ V
-            eo = ep @ V.abs() + (r + f(lk)) * (p @ V.abs())
+            eo = ep @ V.abs() + (rf + f(lk)) * (p @ V.abs())
             res["out"][0][sq, h] += o
             res["out"][1][sq, h] += eo + u * o.abs()
             dp = dO @ V.t()
             delta = (dO * o).sum(1, keepdim=True)
             size = dO.abs() @ V.abs().t() + (dO.abs() * o.abs()).sum(1, keepdim=True)
-            # the kernel's delta starts from the stored, rounded out
-            ed = (dO.abs() * (u * o.abs() + eo)).sum(1, keepdim=True) + f(D) * size
+            ed = (dO.abs() * (2.0 ** -24 * o.abs() + eo)).sum(1, keepdim=True) + f(D) * size
             ds = p * (dp - delta)
             eds = ep * (dp - delta).abs() + p * ed + 4 * 2.0 ** -24 * p * size
             edsr = eds + r * ds.abs()

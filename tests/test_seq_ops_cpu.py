@@ -93,7 +93,7 @@ def test_attention_entry_refuses():
     assert call(a) == -6 and call(a, 4096, need - 1) == -6 and call(a, 4104, need) == -3
     back = dict(lse=4096, dout=4096, dq=4096, dk=4096, dv=4096)
     bwd = lambda a, ws=None, n=0: lib.swr_seq_attention_bwd(C.byref(a), ws, n, None)
-    for want, kw in [(-1, dict(back, lse=None)), (-1, dict(back, dk=None)), (-3, dict(back, dq=4100)), (-6, back)]:
+    for want, kw in [(-1, dict(back, lse=None)), (-1, dict(back, dk=None)), (-1, dict(back, dtype=H.BF16)), (-3, dict(back, dq=4100)), (-6, back)]:
         assert bwd(attention_args(**kw)) == want, kw
     a = attention_args(**back)
     assert bwd(a, 4096, lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a)) - 1) == -6
