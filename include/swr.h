@@ -825,7 +825,8 @@ typedef struct {
     int32_t B, Hq, Hk, D;
     int32_t dtype, causal, max_q, max_k;
     float scale;
-    int32_t n_dist, n_buckets, pad;
+    int32_t n_dist, n_buckets;
+    int32_t accumulate;                /* backward: 1 adds into dbias (gradient arena), 0 overwrites */
     const void* q; int64_t q_row, q_head;
     const void* k; int64_t k_row, k_head;
     const void* v; int64_t v_row, v_head;
@@ -839,7 +840,7 @@ typedef struct {
     const int32_t* buckets;            /* [n_dist] */
     const void* dout; int64_t do_row, do_head;
     void* dq; void* dk; void* dv;
-    float* dbias;                      /* [Hq, n_buckets], nullable, overwritten */
+    float* dbias;                      /* [Hq, n_buckets], nullable */
     uint32_t* err_flag;                /* nullable */
 } swr_seq_attention_args;
 size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_args* a);
@@ -855,12 +856,12 @@ int swr_seq_attention_bwd(const swr_seq_attention_args* a, void* workspace, size
  *   u = z rms(z) w_pre     (w_pre NULL: no u)           z enters unrounded
  * Rows of N <= SWR_NORM_GATE_MAX_WIDTH elements of `dtype` (SWR_F32 / SWR_BF16); x, y, gate, dz, du have leading dimensions, z, u, dx,
  * dy, dgate are contiguous; weights, their gradients and ry / rz ([M], kept for the backward; nullable in a forward without one) fp32.
- * Backward: dz and du nullable (a missing one counts as zeros), dx, dy, dgate overwritten, dw_post / dw_pre nullable, overwritten,
- * fixed-order column sums (workspace needed when one of them is asked for). */
+ * Backward: dz and du nullable (a missing one counts as zeros), dx, dy, dgate overwritten, dw_post / dw_pre nullable, fixed-order
+ * column sums (accumulate = 1 adds into them -- gradient arena; workspace needed when one of them is asked for). */
 #define SWR_NORM_GATE_MAX_WIDTH 8192
 typedef struct {
     int64_t M;
-    int32_t N, dtype;
+    int32_t N, dtype, accumulate, pad;
     float eps, scale;
     const void* x; int64_t ldx;
     const void* y; int64_t ldy;

@@ -22,7 +22,7 @@
 
 struct NgK {
     int64_t M;
-    int N, n_wgs;
+    int N, n_wgs, accumulate;
     float eps, scale;
     const void *x, *y, *gate; int64_t ldx, ldy, ldg;
     const float *w_post, *w_pre;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void norm_gate_dw_kernel(const NgK k) {
     if (grp == 0 && col < k.N) {
         for (int g = 1; g < 16; ++g) s += sm[g][c];
         float* out = w ? k.dw_pre : k.dw_post;
-        if (out) out[col] = static_cast<float>(s);
+        if (out) out[col] = static_cast<float>(k.accumulate ? out[col] + s : s);
     }
 }
 
@@ -306,7 +306,7 @@ static int ng_check(const swr_norm_gate_args* p, bool backward) {
 static NgK ng_args(const swr_norm_gate_args* p, bool backward) {
     NgK k{};
     const int e = p->dtype == SWR_F32 ? 4 : 2;
-    k.M = p->M; k.N = p->N; k.eps = p->eps; k.scale = p->scale;
+    k.M = p->M; k.N = p->N; k.accumulate = p->accumulate; k.eps = p->eps; k.scale = p->scale;
     k.x = p->x; k.y = p->y; k.gate = p->gate; k.ldx = p->ldx; k.ldy = p->ldy; k.ldg = p->ldg;
     k.w_post = p->w_post; k.w_pre = p->w_pre; k.z = p->z; k.u = p->u; k.ry = p->ry; k.rz = p->rz;
     k.dz = p->dz; k.du = p->du; k.lddz = p->lddz; k.lddu = p->lddu;

@@ -37,7 +37,7 @@ struct SaK {
     const uint8_t* key_mask;
     const float* bias; const int32_t* buckets;
     const void* dout; int64_t do_row, do_head;
-    void *dq, *dk, *dv; float* dbias;
+    void *dq, *dk, *dv; float* dbias; int accumulate;
     uint32_t* err_flag;
     // launch geometry
     int tiles, per_unit, units, together;  // column tiles per sequence, workgroups per (sequence, key head), B * Hk, sa_unit

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void seq_attention_dbias_kernel(const SaK a) {
     double s = 0.;
     for (int i = threadIdx.x; i < a.bias_slots; i += 256) s += static_cast<double>(p[i]);
     s = swr_block_sum_f64<256>(s, sm);
-    if (threadIdx.x == 0) a.dbias[blockIdx.x] = static_cast<float>(s);
+    if (threadIdx.x == 0) a.dbias[blockIdx.x] = static_cast<float>(a.accumulate ? a.dbias[blockIdx.x] + s : s);
 }
 
 template <int NP, int DP, int NW, bool FAST>

@@ -332,7 +332,7 @@ SaK sa_args(const swr_seq_attention_args* p) {
     a.out32 = p->dtype == SWR_F32 ? static_cast<float*>(p->out) : p->out32;
     a.out = p->out; a.lse = p->lse; a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.q_len = p->q_len; a.k_len = p->k_len; a.key_mask = p->key_mask;
     a.bias = p->bias; a.buckets = p->buckets; a.dout = p->dout; a.do_row = p->do_row; a.do_head = p->do_head;
-    a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.dbias = p->dbias; a.err_flag = p->err_flag;
+    a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.dbias = p->dbias; a.accumulate = p->accumulate; a.err_flag = p->err_flag;
     a.units = p->B * p->Hk; a.pack = 1; a.splits = 1;
     return a;
 }

@@ -157,7 +157,7 @@ class LayerNormArgs(C.Structure):
 class SeqAttentionArgs(C.Structure):
     _fields_ = [("Tq", C.c_int64), ("Tk", C.c_int64), ("B", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
                 ("dtype", C.c_int32), ("causal", C.c_int32), ("max_q", C.c_int32), ("max_k", C.c_int32), ("scale", C.c_float),
-                ("n_dist", C.c_int32), ("n_buckets", C.c_int32), ("pad", C.c_int32),
+                ("n_dist", C.c_int32), ("n_buckets", C.c_int32), ("accumulate", C.c_int32),
                 ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
                 ("k", C.c_void_p), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v", C.c_void_p), ("v_row", C.c_int64), ("v_head", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
@@ -171,7 +171,7 @@ SEQ_MAX_DIM, SEQ_MAX_DIST, SEQ_MAX_BUCKETS, SEQ_MAX_TABLE = 128, 4097, 256, 8192
 
 
 class NormGateArgs(C.Structure):
-    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float), ("scale", C.c_float),
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32), ("accumulate", C.c_int32), ("pad", C.c_int32), ("eps", C.c_float), ("scale", C.c_float),
                 ("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64), ("gate", C.c_void_p),
                 ("ldg", C.c_int64), ("w_post", C.c_void_p), ("w_pre", C.c_void_p), ("z", C.c_void_p), ("u", C.c_void_p),
                 ("ry", C.c_void_p), ("rz", C.c_void_p), ("dz", C.c_void_p), ("lddz", C.c_int64), ("du", C.c_void_p),

@@ -35,12 +35,17 @@ class SequenceFeature(SparseFeature):
     """Multi-hot / behaviour-sequence column (reference `basic/features.py:5-46`): ids of shape (batch, seq_len), padded;
     `pooling` in "sum" / "mean" / "concat".  Positions equal to `padding_idx` (or to -1 when no padding_idx is given) are
     masked out of the pooled embedding (`basic/layers.py:137-140`).  The lookup is one pooled-gather launch
-    (csrc/embed_bag.hip)."""
+    (csrc/embed_bag.hip).
+
+    `pooling="attention"` (no reference counterpart): the events attend to each other in a `basic.layers.SequenceBlock` -- `attention`
+    holds its keyword arguments, e.g. `{"n_heads": 4, "max_distance": 64}` -- and the mean of the unmasked ones is the column block.
+    Served by `EmbeddingLayer.forward(squeeze_dim=True)`."""
 
     def __init__(self, name, vocab_size, embed_dim=None, pooling="mean", shared_with=None, padding_idx=None,
-                 initializer=RandomNormal(0, 0.0001), hash_seed=0):
+                 initializer=RandomNormal(0, 0.0001), hash_seed=0, attention=None):
         super().__init__(name, vocab_size, embed_dim, shared_with, padding_idx, initializer, hash_seed)
         self.pooling = pooling
+        self.attention = dict(attention or {})
 
     def __repr__(self):
         return f'<SequenceFeature {self.name} with Embedding shape ({self.vocab_size}, {self.embed_dim})>'

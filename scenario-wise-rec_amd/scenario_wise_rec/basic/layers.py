@@ -37,6 +37,10 @@ class EmbeddingLayer(SwrModule):
                 self.embed_dict[fea.name] = fea.get_embedding_layer()
             elif isinstance(fea, DenseFeature):
                 self.n_dense += 1
+        attending = {f.name: SequenceBlock(f.embed_dim, **f.attention) for f in features
+                     if isinstance(f, SequenceFeature) and f.pooling == "attention"}
+        if attending:                            # (no empty container: the other models' module trees stay the reference's)
+            self.seq_blocks = nn.ModuleDict(attending)
 
     def forward(self, x, features, squeeze_dim=False, onehot=False):
         """`onehot=True` (training, squeeze_dim): the caller promises that the returned tensor is consumed by exactly ONE
@@ -45,7 +49,9 @@ class EmbeddingLayer(SwrModule):
         sparse, dense = [], []
         for fea in features:
             if isinstance(fea, SequenceFeature):
-                if fea.pooling not in ("sum", "mean", "concat"):
+                if fea.pooling == "attention" and squeeze_dim and fea.name in getattr(self, "seq_blocks", ()):
+                    onehot = False               # (the consuming layer reads a concatenation, not the lookup's own buffer)
+                elif fea.pooling not in ("sum", "mean", "concat"):
                     raise ValueError("Sequence pooling method supports only pooling in %s, got %s." %
                                      (["sum", "mean"], fea.pooling))
                 sparse.append(fea)               # pooled lookup (`layers.py:73-87`): a column block like any sparse feature
@@ -65,13 +71,33 @@ class EmbeddingLayer(SwrModule):
         _plan_part(plan, weights, {}, self, x, sparse, dense if squeeze_dim else [])
         out = _run_plan(plan, weights)
         if squeeze_dim:
-            return out
+            return self._attend(x, out, sparse) if any(getattr(f, "pooling", None) == "attention" for f in sparse) else out
         if any(b["mode"] == 2 for b in plan.bags):
             raise NotImplementedError("squeeze_dim=False with pooling='concat' ([B, F, L, E]) is not built")
         dims = {s[3] for s in plan.sparse} | {b["dim"] for b in plan.bags}
         if len(dims) != 1:
             raise RuntimeError("squeeze_dim=False needs equal embed_dim for all sparse features")
         return out.reshape(out.shape[0], len(plan.sparse) + len(plan.bags), dims.pop())
+
+
+    def _attend(self, x, out, sparse):
+        """The column blocks of attention-pooled histories, [B, L * E] as looked up, replaced by their [B, E] poolings."""
+        parts, col, start = [], 0, 0
+        for fea in sparse:
+            seq = isinstance(fea, SequenceFeature)
+            L = x[fea.name].shape[1] if seq and fea.pooling in ("concat", "attention") else 1
+            width = self.embed_dict[fea.shared_with if fea.shared_with is not None else fea.name].weight.shape[1] * L
+            if seq and fea.pooling == "attention":
+                if col > start:
+                    parts.append(out[:, start:col])
+                ids = x[fea.name]
+                seen = ids != (-1 if fea.padding_idx is None else fea.padding_idx)
+                parts.append(self.seq_blocks[fea.name].pool(out[:, col:col + width], seen))
+                start = col + width
+            col += width
+        if out.shape[1] > start:
+            parts.append(out[:, start:])
+        return torch.cat(parts, dim=1)
 
 
 def _new_plan(layer):
@@ -101,7 +127,7 @@ def _plan_part(plan, weights, wpos, layer, x, sparse, dense):
             idx = x[fea.name]
             if idx.dim() != 2:
                 raise ValueError(f"sequence feature {fea.name!r}: expected ids of shape (batch_size, seq_len), got {tuple(idx.shape)}")
-            mode = {"sum": 0, "mean": 1, "concat": 2}[fea.pooling]
+            mode = {"sum": 0, "mean": 1, "concat": 2, "attention": 2}[fea.pooling]
             plan.bags.append({"wpos": wpos[key], "idx": idx, "vocab": w.shape[0], "dim": w.shape[1], "col": col,
                               "L": idx.shape[1], "mode": mode, "pad": fea.padding_idx, "seed": getattr(fea, "hash_seed", 0)})
             col += w.shape[1] * (idx.shape[1] if mode == 2 else 1)
@@ -188,6 +214,10 @@ def fused_lookup(x, parts):
     wpos = {}
     for part in parts:
         layer, feats = part[0], part[1]
+        for f in feats:
+            if isinstance(f, SequenceFeature) and f.pooling == "attention":
+                raise NotImplementedError(f"sequence feature {f.name!r}: pooling='attention' is not built for models that look two "
+                                          "feature groups up together (PPNet, EPNet)")
         n0 = len(weights)
         sparse = [f for f in feats if isinstance(f, (SparseFeature, SequenceFeature))]
         dense = [f for f in feats if not isinstance(f, (SparseFeature, SequenceFeature))]
@@ -362,6 +392,57 @@ def mlp_bank_forward(mlps, x, shared_input, first_block=0):
         grouped = not (shared_input and m0.n_blocks == first_block)
         x = LayerBank([m.output_linear() for m in mlps], grouped=grouped)(x, training)
     return x
+
+
+class SequenceBlock(SwrModule):
+    """One self-attention block over behaviour histories (no reference counterpart; the poolings of `basic/layers.py:174-228` drop the
+    order of the events):
+
+        u = norm(x) w_in;   q, k, v = u W_qkv;   a = attention(q, k, v) with a learned bias per head and bucket of the distance
+        z = x + 2 sigmoid(gate(u)) norm(a W_out) w_out
+
+    `n_kv_heads` key / value heads are shared by the `n_heads` query heads.  fp32, like every layer of the package; the norms, gate and
+    residual are one launch each way (ops.norm_gate_residual), the attention one forward and three or four backward
+    (ops.seq_attention)."""
+
+    def __init__(self, dim, n_heads=4, n_kv_heads=None, n_buckets=16, max_distance=64, causal=True, eps=1e-6):
+        super().__init__()
+        n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if dim % n_heads or n_heads % n_kv_heads:
+            raise ValueError(f"SequenceBlock: {dim} columns, {n_heads} heads over {n_kv_heads} key heads")
+        self.dim, self.n_heads, self.n_kv_heads, self.head_dim = dim, n_heads, n_kv_heads, dim // n_heads
+        self.causal, self.eps = bool(causal), float(eps)
+        self.norm_in, self.norm_out = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
+        self.qkv = nn.Linear(dim, (n_heads + 2 * n_kv_heads) * self.head_dim, bias=False)
+        self.out = nn.Linear(dim, dim, bias=False)
+        self.gate = GateNU(dim, dim)
+        self.position = nn.Parameter(torch.zeros(n_heads, n_buckets))
+        self.register_buffer("buckets", ops.seq_buckets(n_buckets, max_distance, self.causal, device="cpu"), persistent=False)
+
+    def forward(self, x, cu, max_len=None, key_mask=None, length=None):
+        """x [T, dim]: packed events; cu (int32, [sequences + 1]): their prefix sums; key_mask ([T]) / length (int32, [sequences]): events
+        that count, as `ops.seq_attention` takes them."""
+        H, Hk, D = self.n_heads, self.n_kv_heads, self.head_dim
+        u = ops.norm_gate_residual(x, w_pre=self.norm_in, eps=self.eps)
+        qkv = LayerBank([self.qkv])(u, self.training).view(-1, H + 2 * Hk, D)
+        a = ops.seq_attention(qkv[:, :H], qkv[:, H:H + Hk], qkv[:, H + Hk:], cu, max_q=max_len, causal=self.causal, bias=self.position,
+                              buckets=self.buckets, key_mask=key_mask, q_len=length)
+        o = LayerBank([self.out])(a.reshape(-1, self.dim), self.training)
+        return ops.norm_gate_residual(x, o, gate=self.gate.logits(u), w_post=self.norm_out, scale=self.gate.gemma, eps=self.eps)
+
+    def pool(self, emb, seen):
+        """emb [B, L * dim]: the padded events of B histories; seen [B, L] bool: those that count.  -> [B, dim], the mean of the seen
+        events' rows behind the block, zeros where there is none."""
+        B, L = seen.shape
+        if B * L == 0:
+            return emb.new_zeros((B, self.dim))
+        cu = torch.arange(0, (B + 1) * L, L, dtype=torch.int32, device=emb.device)
+        mask = seen.reshape(-1)
+        z = self(emb.reshape(B * L, self.dim), cu, L, mask).view(-1, self.n_heads, self.head_dim)
+        # the mean of the seen rows is attention with equal scores: one query of zeros for each history
+        one = torch.arange(B + 1, dtype=torch.int32, device=emb.device)
+        q = torch.zeros((B, self.n_heads, self.head_dim), dtype=z.dtype, device=z.device)
+        return ops.seq_attention(q, z.detach(), z, one, cu, max_q=1, max_k=L, causal=False, key_mask=mask).reshape(B, self.dim)
 
 
 class GateNU(SwrModule):

@@ -2790,6 +2790,7 @@ class SeqAttention(Function):
             return q.new_zeros(q.shape)
         out, lse, out32, ctx.args = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         # (ctx.args: addresses of what is kept here)
+        ctx.bias = bias
         ctx.save_for_backward(q, k, v, bias, out32, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         return out
 
@@ -2803,14 +2804,18 @@ class SeqAttention(Function):
         dev = q.device
         dout = _unit_last(dout if dout.dtype == q.dtype else dout.to(q.dtype))
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        dbias = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[4] else None
+        direct = _grad_alias((ctx.bias,)) if bias is not None and ctx.needs_input_grad[4] else None       # (gradient arena: added in place)
+        dbias = direct if direct is not None else (torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[4] else None)
         a = ctx.args
         a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.dbias = None if dbias is None else dbias.data_ptr()
+        a.dbias, a.accumulate = (None if dbias is None else dbias.data_ptr()), int(direct is not None)
         nbytes = lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _launch(lib.swr_seq_attention_bwd, "swr_seq_attention_bwd", q, C.byref(a), H.ptr(ws), nbytes)
+        if direct is not None:
+            _mark_touched((ctx.bias,))
+            dbias = None
         need = ctx.needs_input_grad
         return None, dq if need[1] else None, dk if need[2] else None, dv if need[3] else None, dbias, None, None, None, None, None, None
 
@@ -2921,7 +2926,7 @@ class NormGateResidual(Function):
     def forward(ctx, meta, x, y, gate, w_post, w_pre):
         ctx.set_materialize_grads(False)
         z, u, ry, rz = NormGateResidual.launch(True, meta, x, y, gate, w_post, w_pre)
-        ctx.meta = meta
+        ctx.meta, ctx.weights = meta, (w_post, w_pre)
         ctx.save_for_backward(x, y, gate, w_post, w_pre, ry, rz)
         return z, u
 
@@ -2937,7 +2942,11 @@ class NormGateResidual(Function):
         dev, M, N = x.device, x.shape[0], x.shape[1]
         empty = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
         dx, dy, dg = empty(x), empty(y), empty(gate)
-        dwp, dwn = empty(w_post) if need[4] else None, empty(w_pre) if need[5] else None
+        # weights' gradients: added to the gradient arena where both have a place of their own there, else returned
+        want = [w if w is not None and n else None for w, n in zip(ctx.weights, (need[4], need[5] and du is not None))]
+        alias = [None if w is None else _grad_alias((w,)) for w in want]
+        direct = any(w is not None for w in want) and all((w is None) == (g is None) for w, g in zip(want, alias)) and want[0] is not want[1]
+        dwp, dwn = alias if direct else (empty(w) for w in want)
         a = _norm_gate_args(ctx.meta, x, y, gate, w_post, w_pre, ry, rz)
         if dz is not None:
             dz = _unit_last(dz if dz.dtype == x.dtype else dz.to(x.dtype))
@@ -2945,13 +2954,16 @@ class NormGateResidual(Function):
         if du is not None:
             du = _unit_last(du if du.dtype == x.dtype else du.to(x.dtype))
             a.du, a.lddu = du.data_ptr(), du.stride(0)
-        a.dx = dx.data_ptr()
+        a.dx, a.accumulate = dx.data_ptr(), int(direct)
         for name, t in (("dy", dy), ("dgate", dg), ("dw_post", dwp), ("dw_pre", dwn)):
             if t is not None:
                 setattr(a, name, t.data_ptr())
         nbytes = lib.swr_norm_gate_bwd_workspace_bytes(M, N) if dwp is not None or dwn is not None else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _launch(lib.swr_norm_gate_bwd, "swr_norm_gate_bwd", x, C.byref(a), H.ptr(ws), nbytes)
+        if direct:
+            _mark_touched([w for w in want if w is not None])
+            dwp = dwn = None
         return None, dx if need[1] else None, dy if need[2] else None, dg if need[3] else None, dwp, dwn
 
 

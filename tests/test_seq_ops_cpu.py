@@ -117,3 +117,16 @@ def test_norm_entry_refuses():
                      (-1, dict(back, gate=4096)), (-1, dict(back, w_post=4096)), (-6, dict(back, w_post=4096, ry=4096, dw_post=4096))]:
         assert lib.swr_norm_gate_bwd(C.byref(args(**kw)), None, 0, None) == want, kw
     assert lib.swr_norm_gate_bwd_workspace_bytes(8, 8193) == 0 and lib.swr_norm_gate_bwd_workspace_bytes(100, 64) > 0
+
+
+def test_only_attention_pooling_adds_parameters():
+    from scenario_wise_rec.basic.features import SequenceFeature, SparseFeature
+    from scenario_wise_rec.basic.layers import EmbeddingLayer
+    plain = EmbeddingLayer([SparseFeature("a", 5, 4), SequenceFeature("h", 7, 4, pooling="mean")])
+    assert sorted(plain.state_dict()) == ["embed_dict.a.weight", "embed_dict.h.weight"]
+    att = EmbeddingLayer([SequenceFeature("h", 7, 8, pooling="attention", attention={"n_heads": 2, "n_buckets": 4, "max_distance": 9})])
+    keys = sorted(k for k in att.state_dict() if k.startswith("seq_blocks.h."))
+    assert [k[len("seq_blocks.h."):] for k in keys] == [
+        "gate.network.0.bias", "gate.network.0.weight", "gate.network.2.bias", "gate.network.2.weight", "norm_in", "norm_out",
+        "out.weight", "position", "qkv.weight"]
+    assert tuple(att.state_dict()["seq_blocks.h.position"].shape) == (2, 4)
