@@ -149,6 +149,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 const int k0 = t * KT + kb * 32;
                 if (wfirst > wlast || k0 >= sq.lk || (a.causal && k0 > wlast + sq.shift)) continue;      // (whole waves)
                 ln.fresh();
+                sa_prio<NP == 1 && NW == 4>(1);
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
@@ -159,6 +160,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                     dP = sa_mma(A, dO[s], dP);
                 }
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
+                sa_prio<NP == 1 && NW == 4>(0);
                 const SaSpan sp = sa_span(a, near_d, far_d);
                 if (sp.apart) {
                     const float add = (a.row ? bt[sp.entry] : 0.f) - lse;
@@ -209,6 +211,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                         else acc[a.causal ? dist : dist + a.reach] += sum;
                     }
                 }
+                sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
@@ -223,6 +226,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                         dQ[db] = sa_mma(A, P, dQ[db]);
                     }
                 }
+                sa_prio<NP == 1 && NW == 4>(0);
             }
         }
         if (exists) {
@@ -375,6 +379,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 const int r0 = q0 + rb * 32, rlast = min(r0 + 31, sq.lq - 1);
                 if (r0 >= sq.lq || (a.causal && rlast + sq.shift < wfirst)) continue;
                 ln.fresh();
+                sa_prio<NP == 1 && NW == 4>(1);
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
@@ -389,6 +394,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
                 // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
                 // behind the last query have lse = +inf, p = 0)
+                sa_prio<NP == 1 && NW == 4>(0);
                 const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
                 const float *lr = lse_s + rb * 32 + 4 * hi, *dr = delta_s + rb * 32 + 4 * hi;
                 if (sp.apart) {
@@ -403,6 +409,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
+                sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
@@ -424,6 +431,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                         dK[db] = sa_mma(A, P, dK[db]);
                     }
                 }
+                sa_prio<NP == 1 && NW == 4>(0);
             }
         }
         if (exists) {

@@ -133,6 +133,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             if (wfirst > wlast || (a.causal && k0 > wlast + sq.shift)) continue;
 
             ln.fresh();
+            sa_prio<NP == 1 && NW == 4>(1);
             f32x16 S[KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -146,6 +147,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             }
             // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
             // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
+            sa_prio<NP == 1 && NW == 4>(0);
             const float* bh = bt + hsub * a.row;
             float mul[KB], add[KB], mx = -INFINITY;
 #pragma unroll
@@ -208,6 +210,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 }
                 l += sum;
             }
+            sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
             for (int ks = 0; ks < KT / 16; ++ks) {
                 float pf[8];
@@ -222,6 +225,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                     O[db] = sa_mma(A, P, O[db]);
                 }
             }
+            sa_prio<NP == 1 && NW == 4>(0);
         }
         l += __shfl_xor(l, 32);
         if (!live) {                           // a column without a query went through the products as a row of zeros
