@@ -807,7 +807,9 @@ int swr_block_select_bwd(const float* dout, int64_t ldo, const void* domain, int
  * counterpart: the reference pools a history by sum / mean / concat, basic/layers.py:174-228).
  *   s_ij = scale q_i . k_j + bias[h, buckets[entry(i + lk - lq - j)]]      i < lq, j < lk of one sequence, h = query head
  *   out_i = sum_j softmax_j(s_ij) v_j over the allowed j: key_mask[j] != 0 and, causal, j <= i + lk - lq
- * A row with no allowed key is zeros, and so are its gradients.  Query head h reads key head h / (Hq / Hk).
+ * A row with no allowed key is zeros, and so are its gradients.  Query head h reads key head h / (Hq / Hk).  Values in use are
+ * expected to be finite: what is hidden by key_mask or lies beyond the lengths may be anything, but a NaN or infinity behind the
+ * causal border enters products with zeros and may spread to earlier rows of its sequence.
  * Sequence b: query rows cu_q[b] .. cu_q[b + 1], key rows cu_k[b] .. cu_k[b + 1] (prefix sums, int32, B + 1 entries); q_len / k_len
  * (nullable, [B]) = how many of them are in use.  Rows that are in no sequence or not in use come out as zeros.  A prefix or length
  * outside its range is clamped and raises SWR_FLAG_INDEX_OOR, as does a bucket outside [0, n_buckets).
@@ -817,9 +819,9 @@ int swr_block_select_bwd(const float* dout, int64_t ldo, const void* domain, int
  * max_q / max_k: longest sequence -- they choose the launch and its tiling (right for any value, other values round differently).
  * Deterministic: fixed summation orders, no atomics on results. */
 #define SWR_SEQ_MAX_DIM 128
-#define SWR_SEQ_MAX_DIST 4097
+#define SWR_SEQ_MAX_DIST 2049
 #define SWR_SEQ_MAX_BUCKETS 256
-#define SWR_SEQ_MAX_TABLE 8192          /* n_dist * (Hq / Hk): the bias rows of a group are held in LDS */
+#define SWR_SEQ_MAX_TABLE 12288         /* (n_dist + 132) * (Hq / Hk): the bias rows of a group are held in LDS */
 typedef struct {
     int64_t Tq, Tk;                    /* rows of q / out and of k / v */
     int32_t B, Hq, Hk, D;

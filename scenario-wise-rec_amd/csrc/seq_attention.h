@@ -41,6 +41,7 @@ struct SaK {
     uint32_t* err_flag;
     // launch geometry
     int tiles, per_unit, units, together;  // column tiles per sequence, workgroups per (sequence, key head), B * Hk, sa_unit
+    int rest;                              // units behind the last: they write the rows of no sequence
     int pack;                              // query heads side by side in the columns (1 or G)
     int splits;                            // workgroups per key range
     float* part;                           // forward, splits > 1: [splits][Hq][Tq] (max, sum), then [splits][Hq][Tq][D]
@@ -116,14 +117,6 @@ __device__ __forceinline__ f32x16 sa_mma(const bf16x8 (&a)[3], const bf16x8 (&b)
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
-}
-// A wave in its products goes before the SIMD's other wave in its exponentials (bf16, four waves: packed training step 0.95 -> 0.92 ms,
-// prompts 2.39 -> 2.35 ms; the small forms lose 1 % and do without).
-template <bool ON>
-__device__ __forceinline__ void sa_prio(int on) {
-    if (!ON) return;
-    if (on) __builtin_amdgcn_s_setprio(1);
-    else __builtin_amdgcn_s_setprio(0);
 }
 __device__ __forceinline__ f32x16 sa_zero16() {
     f32x16 z;
@@ -376,30 +369,32 @@ __device__ __forceinline__ float sa_bias2(float b) {
 }
 __device__ __forceinline__ int sa_bucket(const SaK& a, int i) { return max(0, min(a.buckets[i], a.n_buckets - 1)); }
 // rows of heads h .. h + heads - 1.  A value is two loads deep (bucket, bias) and a single token's whole work is a few loads deep: every
-// thread has the buckets of eight entries in flight, then their values (one entry after the other took 15 of the 60 us of a chunk of
-// 13 tokens over 32 caches).
-__device__ __forceinline__ void sa_bias_rows(const SaK& a, int h, int heads, float* rows, int nthreads) {
+// thread has the buckets of several entries in flight, then their values (one wave, 193 entries, one after the other: the query pass of
+// 1 024 histories up to 50 took 61 us, so 49).
+template <int NT>
+__device__ __forceinline__ void sa_bias_rows(const SaK& a, int h, int heads, float* rows) {
+    constexpr int U = 512 / NT;
     const int low = a.causal ? 0 : -a.reach, n = heads * a.row;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * nthreads) {
-        int d[8], at[8];
-        float x[8];
+    for (int i0 = threadIdx.x; i0 < n; i0 += U * NT) {
+        int d[U], at[U];
+        float x[U];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = min(i0 + u * nthreads, n - 1), hh = i / a.row;
+        for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + u * NT, n - 1), hh = i / a.row;
             d[u] = i - hh * a.row - SA_PAD + low;
             at[u] = (h + hh) * a.n_buckets;
             x[u] = 0.f;
         }
         if (a.n_dist) {
-            int bu[8];
+            int bu[U];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) bu[u] = a.buckets[max(low, min(d[u], a.reach)) - low];
+            for (int u = 0; u < U; ++u) bu[u] = a.buckets[max(low, min(d[u], a.reach)) - low];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = a.bias[at[u] + max(0, min(bu[u], a.n_buckets - 1))];
+            for (int u = 0; u < U; ++u) x[u] = a.bias[at[u] + max(0, min(bu[u], a.n_buckets - 1))];
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (i0 + u * nthreads < n) rows[i0 + u * nthreads] = a.causal && d[u] < 0 ? -INFINITY : sa_bias2(x[u]);
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * NT < n) rows[i0 + u * NT] = a.causal && d[u] < 0 ? -INFINITY : sa_bias2(x[u]);
     }
 }
 // what a block whose distances span near .. far needs: 0 = one value (at .x of the row), 1 = the row
@@ -417,10 +412,17 @@ __device__ __forceinline__ int sa_entry(const SaK& a, int d) { return d + SA_PAD
 __device__ __forceinline__ bool sa_masked(const uint8_t* km, int i) {
     return ((*reinterpret_cast<const uint32_t*>(km + 8 * (i >> 2)) >> (8 * (i & 3))) & 0xff) == 0;
 }
-// rows outside every sequence (before the first, behind the last) are zeros in every output
+// rows outside every sequence (before the first, behind the last) are zeros in every output: the work of the units behind the last
+// one.  base is 16-byte aligned; the edges of a span that is not go 2 bytes at a time.
 __device__ __forceinline__ void sa_zero_rows(void* base, int elem, int64_t r0, int64_t r1, int64_t row_elems, int nthreads, int part, int parts) {
     char* p = static_cast<char*>(base);
     const int64_t n0 = r0 * row_elems * elem, n1 = r1 * row_elems * elem;
-    for (int64_t i = n0 + 2 * (static_cast<int64_t>(part) * nthreads + threadIdx.x); i < n1; i += 2ll * nthreads * parts)
-        *reinterpret_cast<uint16_t*>(p + i) = 0;
+    if (n0 >= n1) return;
+    const int64_t a0 = min((n0 + 15) & ~15ll, n1), a1 = max(n1 & ~15ll, a0);
+    if (part == 0) {
+        for (int64_t i = n0 + 2 * threadIdx.x; i < a0; i += 2 * nthreads) *reinterpret_cast<uint16_t*>(p + i) = 0;
+        for (int64_t i = a1 + 2 * threadIdx.x; i < n1; i += 2 * nthreads) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    }
+    for (int64_t i = a0 + 16 * (static_cast<int64_t>(part) * nthreads + threadIdx.x); i < a1; i += 16ll * nthreads * parts)
+        *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
 }

@@ -57,11 +57,12 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
-    if (unit > a.units) return;
-    if (unit == a.units) {                     // rows of no sequence
+    if (unit >= a.units) {                     // rows of no sequence
+        if (unit >= a.units + a.rest) return;
+        const int part = (unit - a.units) * a.per_unit + within, parts = a.rest * a.per_unit;
         const int64_t end0 = sa_clamp(a.cu_q[0], 0, a.Tq), beg1 = sa_clamp(a.cu_q[a.B], end0, a.Tq), row = static_cast<int64_t>(a.Hq) * a.D;
-        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, 0, end0, row, NT, within, a.per_unit);
-        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, beg1, a.Tq, row, NT, within, a.per_unit);
+        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, 0, end0, row, NT, part, parts);
+        sa_zero_rows(a.dq, NP == 3 ? 4 : 2, beg1, a.Tq, row, NT, part, parts);
         return;
     }
     const int b = unit / a.Hk, hk = unit % a.Hk, g = within % a.G, h = hk * a.G + g, tile0 = a.tiles - 1 - within / a.G;
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
         delta += __shfl_xor(delta, 32);
         const float lse = live ? n->lse[at] : INFINITY;
         if (tile == tile0) {
-            sa_bias_rows(a, h, 1, bt, NT);
+            sa_bias_rows<NT>(a, h, 1, bt);
             if (a.bias_part) {
                 for (int i = lane; i < SA_SKEW / 4; i += 64) reinterpret_cast<float4*>(skew)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
@@ -149,7 +150,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 const int k0 = t * KT + kb * 32;
                 if (wfirst > wlast || k0 >= sq.lk || (a.causal && k0 > wlast + sq.shift)) continue;      // (whole waves)
                 ln.fresh();
-                sa_prio<NP == 1 && NW == 4>(1);
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
@@ -160,7 +160,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                     dP = sa_mma(A, dO[s], dP);
                 }
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
-                sa_prio<NP == 1 && NW == 4>(0);
                 const SaSpan sp = sa_span(a, near_d, far_d);
                 if (sp.apart) {
                     const float add = (a.row ? bt[sp.entry] : 0.f) - lse;
@@ -211,7 +210,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                         else acc[a.causal ? dist : dist + a.reach] += sum;
                     }
                 }
-                sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
@@ -226,7 +224,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                         dQ[db] = sa_mma(A, P, dQ[db]);
                     }
                 }
-                sa_prio<NP == 1 && NW == 4>(0);
             }
         }
         if (exists) {
@@ -295,13 +292,14 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
-    if (unit > a.units) return;
-    if (unit == a.units) {                     // rows of no sequence
+    if (unit >= a.units) {                     // rows of no sequence
+        if (unit >= a.units + a.rest) return;
+        const int part = (unit - a.units) * a.per_unit + within, parts = a.rest * a.per_unit;
         const int64_t end0 = sa_clamp(a.cu_k[0], 0, a.Tk), beg1 = sa_clamp(a.cu_k[a.B], end0, a.Tk), row = static_cast<int64_t>(a.Hk) * a.D;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, 0, end0, row, NT, within, a.per_unit);
-            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, beg1, a.Tk, row, NT, within, a.per_unit);
+            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, 0, end0, row, NT, part, parts);
+            sa_zero_rows(w ? a.dv : a.dk, NP == 3 ? 4 : 2, beg1, a.Tk, row, NT, part, parts);
         }
         return;
     }
@@ -357,7 +355,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
         SaRows<NP, DP, FAST, Cfg::LATE> K, V;
         K.load(kv->k, row * kv->k_row + hk * kv->k_head, live, kv->D, kv->vk, lane);
         if (!Cfg::VL) V.load(kv->v, row * kv->v_row + hk * kv->v_head, live, kv->D, kv->vv, lane);
-        if (tile == within) sa_bias_rows(a, hk * a.G, a.G, tables, NT);
+        if (tile == within) sa_bias_rows<NT>(a, hk * a.G, a.G, tables);
         for (int step = 0; step < steps; ++step) {
             const int q0 = (r_begin + step % n_r) * RT, buf = Cfg::DMA ? step & 1 : 0;
             const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
@@ -379,7 +377,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 const int r0 = q0 + rb * 32, rlast = min(r0 + 31, sq.lq - 1);
                 if (r0 >= sq.lq || (a.causal && rlast + sq.shift < wfirst)) continue;
                 ln.fresh();
-                sa_prio<NP == 1 && NW == 4>(1);
                 f32x16 S = sa_zero16(), dP = sa_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) {
@@ -394,7 +391,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
                 // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
                 // behind the last query have lse = +inf, p = 0)
-                sa_prio<NP == 1 && NW == 4>(0);
                 const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
                 const float *lr = lse_s + rb * 32 + 4 * hi, *dr = delta_s + rb * 32 + 4 * hi;
                 if (sp.apart) {
@@ -409,7 +405,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
-                sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
@@ -431,7 +426,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                         dK[db] = sa_mma(A, P, dK[db]);
                     }
                 }
-                sa_prio<NP == 1 && NW == 4>(0);
             }
         }
         if (exists) {

@@ -41,16 +41,17 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
 
     int within;
     const int unit = sa_unit(blockIdx.x, a.per_unit, a.together, within);
-    if (unit > a.units) return;
-    if (unit == a.units) {                     // rows of no sequence
+    if (unit >= a.units) {                     // rows of no sequence
+        if (unit >= a.units + a.rest) return;
+        const int part = (unit - a.units) * a.per_unit + within, parts = a.rest * a.per_unit;
         const int64_t end0 = sa_clamp(a.cu_q[0], 0, a.Tq), beg1 = sa_clamp(a.cu_q[a.B], end0, a.Tq);
         if (a.splits == 1) {
             const int64_t row = static_cast<int64_t>(a.Hq) * a.D;
-            sa_zero_rows(a.out, NP == 3 ? 4 : 2, 0, end0, row, NT, within, a.per_unit);
-            sa_zero_rows(a.out, NP == 3 ? 4 : 2, beg1, a.Tq, row, NT, within, a.per_unit);
+            sa_zero_rows(a.out, NP == 3 ? 4 : 2, 0, end0, row, NT, part, parts);
+            sa_zero_rows(a.out, NP == 3 ? 4 : 2, beg1, a.Tq, row, NT, part, parts);
         }
         const int64_t n_tail = end0 + a.Tq - beg1, heads = static_cast<int64_t>(a.Hq) * (a.splits > 1 ? a.splits : 1);
-        for (int64_t i = static_cast<int64_t>(within) * NT + threadIdx.x; i < n_tail * heads; i += static_cast<int64_t>(a.per_unit) * NT) {
+        for (int64_t i = static_cast<int64_t>(part) * NT + threadIdx.x; i < n_tail * heads; i += static_cast<int64_t>(parts) * NT) {
             const int64_t h = i / n_tail, r = i % n_tail, at = h * a.Tq + (r < end0 ? r : beg1 + r - end0);
             if (a.splits > 1) { a.part[2 * at] = -INFINITY; a.part[2 * at + 1] = 0.f; }
             else if (a.lse) a.lse[at] = INFINITY;
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
         for (int db = 0; db < DP / 32; ++db) O[db] = sa_zero16();
         float m = -INFINITY, l = 0.f;
 
-        if (tile == tile0) sa_bias_rows(a, h0, a.pack, bt, NT);
+        if (tile == tile0) sa_bias_rows<NT>(a, h0, a.pack, bt);
         for (int t = t0; t < t1; ++t) {
             const int buf = Cfg::DMA ? (t - t0) & 1 : 0;
             const sa_lds kt = (sa_lds)smem + buf * 2 * TILE, vt = kt + TILE;
@@ -133,7 +134,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             if (wfirst > wlast || (a.causal && k0 > wlast + sq.shift)) continue;
 
             ln.fresh();
-            sa_prio<NP == 1 && NW == 4>(1);
             f32x16 S[KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -147,7 +147,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             }
             // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
             // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
-            sa_prio<NP == 1 && NW == 4>(0);
             const float* bh = bt + hsub * a.row;
             float mul[KB], add[KB], mx = -INFINITY;
 #pragma unroll
@@ -210,7 +209,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 }
                 l += sum;
             }
-            sa_prio<NP == 1 && NW == 4>(1);
 #pragma unroll
             for (int ks = 0; ks < KT / 16; ++ks) {
                 float pf[8];
@@ -225,7 +223,6 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                     O[db] = sa_mma(A, P, O[db]);
                 }
             }
-            sa_prio<NP == 1 && NW == 4>(0);
         }
         l += __shfl_xor(l, 32);
         if (!live) {                           // a column without a query went through the products as a row of zeros
@@ -307,8 +304,12 @@ int sa_check(const swr_seq_attention_args* p, bool backward) {
     if (p->n_dist) {
         SWR_REQUIRE(p->bias && p->buckets && p->n_buckets >= 1, SWR_ERR_ARG);
         SWR_REQUIRE(p->n_dist <= SWR_SEQ_MAX_DIST && p->n_buckets <= SWR_SEQ_MAX_BUCKETS && (p->causal || p->n_dist % 2 == 1), SWR_ERR_UNSUPPORTED);
-        SWR_REQUIRE(static_cast<int64_t>(p->n_dist) * (p->Hq / p->Hk) <= SWR_SEQ_MAX_TABLE, SWR_ERR_UNSUPPORTED);
+
     }
+    // (the bias rows of a group and the per-distance sums have their place in LDS beside the tiles)
+    const int64_t reach = p->n_dist ? (p->causal ? p->n_dist - 1 : p->n_dist / 2) : 0;
+    SWR_REQUIRE(static_cast<int64_t>(sa_row_entries(p->n_dist, static_cast<int>(reach), p->causal)) * (p->Hq / p->Hk) <= SWR_SEQ_MAX_TABLE, SWR_ERR_UNSUPPORTED);
+    SWR_REQUIRE(static_cast<int64_t>(p->B) * p->Hk < (1ll << 30), SWR_ERR_UNSUPPORTED);
     SWR_REQUIRE(((reinterpret_cast<uintptr_t>(p->out) | reinterpret_cast<uintptr_t>(p->out32)) & 15) == 0, SWR_ERR_ALIGN);
     if (backward) {
         SWR_REQUIRE(p->lse && (p->out32 || p->dtype == SWR_F32) && p->dout && p->dq && p->dk && p->dv, SWR_ERR_ARG);
@@ -350,9 +351,10 @@ int sa_waves(int64_t columns, const SaK& a, bool fp32) {
     return columns <= 32 ? 1 : (columns <= 64 ? 2 : 4);
 }
 
-// workgroups of a launch (the rows of no sequence are one more unit), or 0 when they do not fit a grid
+// workgroups of a launch, or 0 when they do not fit a grid.  The rows of no sequence get units for at least 256 workgroups of their own.
 unsigned sa_grid(SaK& a) {
-    const int64_t each = (static_cast<int64_t>(a.units) + 1 + 7) / 8;               // units per XCD
+    a.rest = (256 + a.per_unit - 1) / a.per_unit;
+    const int64_t each = (static_cast<int64_t>(a.units) + a.rest + 7) / 8;          // units per XCD
     if (a.together <= 0 || a.together > each) a.together = static_cast<int>(each);
     const int64_t slots = (each + a.together - 1) / a.together * a.together;
     const int64_t max_per_unit = ((1ll << 30) / 8) / slots;

@@ -167,7 +167,7 @@ class SeqAttentionArgs(C.Structure):
                 ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dbias", C.c_void_p), ("err_flag", C.c_void_p)]
 
 
-SEQ_MAX_DIM, SEQ_MAX_DIST, SEQ_MAX_BUCKETS, SEQ_MAX_TABLE = 128, 4097, 256, 8192        # SWR_SEQ_MAX_*
+SEQ_MAX_DIM, SEQ_MAX_DIST, SEQ_MAX_BUCKETS, SEQ_MAX_TABLE = 128, 2049, 256, 12288        # SWR_SEQ_MAX_*
 
 
 class NormGateArgs(C.Structure):

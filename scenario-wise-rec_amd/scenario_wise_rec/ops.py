@@ -2773,7 +2773,7 @@ class SeqAttention(Function):
 
     @staticmethod
     def launch(want, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
-        """-> out, what the backward needs besides (None unless `want`), the argument block."""
+        """-> out, and what the backward needs besides: lse (None unless `want`), the unrounded rows."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
         out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want and q.dtype != torch.float32 else None
@@ -2781,16 +2781,15 @@ class SeqAttention(Function):
         nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         _launch(lib.swr_seq_attention_fwd, "swr_seq_attention_fwd", q, C.byref(a), H.ptr(ws), nbytes)
-        return out, lse, out if out32 is None else out32, a
+        return out, lse, out if out32 is None else out32
 
     @staticmethod
     def forward(ctx, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
         if q.numel() == 0 or k.numel() == 0:                       # no query, or no key that any query could see
             ctx.save_for_backward(q, k, v, bias)
             return q.new_zeros(q.shape)
-        out, lse, out32, ctx.args = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
-        # (ctx.args: addresses of what is kept here)
-        ctx.bias = bias
+        out, lse, out32 = SeqAttention.launch(True, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
+        ctx.meta, ctx.bias = meta, bias
         ctx.save_for_backward(q, k, v, bias, out32, lse, cu_q, cu_k, q_len, k_len, key_mask, buckets)
         return out
 
@@ -2800,13 +2799,13 @@ class SeqAttention(Function):
         if len(ctx.saved_tensors) == 4:
             return (None,) + tuple(torch.zeros_like(t) if t is not None and n else None
                                    for t, n in zip(ctx.saved_tensors, ctx.needs_input_grad[1:5])) + (None,) * 6
-        q, k, v, bias, _out32, _lse, *_index = ctx.saved_tensors      # (all of it is in ctx.args by address)
+        q, k, v, bias, out32, lse, *index = ctx.saved_tensors
         dev = q.device
         dout = _unit_last(dout if dout.dtype == q.dtype else dout.to(q.dtype))
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         direct = _grad_alias((ctx.bias,)) if bias is not None and ctx.needs_input_grad[4] else None       # (gradient arena: added in place)
         dbias = direct if direct is not None else (torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[4] else None)
-        a = ctx.args
+        a = _seq_args(ctx.meta, q, k, v, out32, lse, out32, index[0], index[1], index[2], index[3], index[4], bias, index[5])
         a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         a.dbias, a.accumulate = (None if dbias is None else dbias.data_ptr()), int(direct is not None)
@@ -2838,7 +2837,8 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
     causal: query i of a sequence sees its keys j <= i + (keys - queries) -- the last query stands at the last key, so one call serves
     training, a whole prompt, and a few new tokens over cached keys.  key_mask (bool / uint8, [Tk]): 0 hides a key from every query.
     bias (fp32, [Hq, n_buckets]) with buckets (`seq_buckets`): a learned bias per head and bucket of the distance i + (keys - queries) - j.
-    max_q / max_k: the longest sequence if known on the host (chooses the launch and its tiling, right for any value; default: all rows).
+    max_q / max_k: the longest sequence if known on the host (chooses the launch and its tiling, right for any value; default: four
+    times the mean).
 
     A row without a visible key, and rows of no sequence or beyond q_len, are zeros with zero gradients; keys beyond k_len or hidden
     by key_mask may hold anything.  Differentiable in q, k, v and bias, deterministic.  Bad prefix sums, lengths and bucket ids are
@@ -2879,12 +2879,11 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
         buckets = _index_vector(buckets, "buckets", buckets.numel(), q.device)
         if not 1 <= buckets.numel() <= H.SEQ_MAX_DIST or (not causal and buckets.numel() % 2 == 0):
             raise ValueError(f"seq_attention: {buckets.numel()} bucket entries (at most {H.SEQ_MAX_DIST}, odd when not causal)")
-        if buckets.numel() * (Hq // Hk) > H.SEQ_MAX_TABLE:
-            raise ValueError(f"seq_attention: {buckets.numel()} bucket entries x {Hq // Hk} heads of a group (at most {H.SEQ_MAX_TABLE})")
         bias = bias.contiguous()
+    # a longest sequence the host does not know: four times the mean (longer ones are walked in more rounds)
+    longest = lambda given, rows: min(rows, 4 * -(-rows // max(n, 1)) if given is None else int(given))
     meta = {"causal": bool(causal), "scale": float(D ** -0.5 if scale is None else scale),
-            "max_q": q.shape[0] if max_q is None else min(int(max_q), q.shape[0]),
-            "max_k": k.shape[0] if max_k is None else min(int(max_k), k.shape[0])}
+            "max_q": longest(max_q, q.shape[0]), "max_k": longest(max_k, k.shape[0])}
     args = (meta, _unit_last(q), _unit_last(k), _unit_last(v), bias, cu_q, cu_k, q_len, k_len, key_mask, buckets)
     if not _needs_grad(q, k, v, bias) and q.numel() and k.numel():
         return SeqAttention.launch(False, *args)[0]               # (serving: without the tape's bookkeeping)

@@ -103,6 +103,22 @@ def test_extreme_rows():
     assert got["u"][4].isnan().all() and got["z"][4].isnan().sum() == 1
 
 
+def test_one_weight_in_both_places():
+    """The same parameter behind the block and before the next: its gradient is the sum of both."""
+    from scenario_wise_rec import ops
+    t, dz, du = make(70, 96, F32, ("y", "w_post"), 6)
+    w = t["w_post"].clone().requires_grad_(True)
+    z, u = ops.norm_gate_residual(t["x"], t["y"], w_post=w, w_pre=w, scale=0.7)
+    got = torch.autograd.grad((z, u), w, (dz, du))[0]
+    want = ref.norm_gate(t["x"], t["y"], None, t["w_post"], t["w_post"], 0.7, 1e-6, dz, du)
+    ref.check(got, tuple(a + b for a, b in zip(want["dw_post"], want["dw_pre"])), "dw")
+    w2 = t["w_post"].clone().requires_grad_(True)
+    w2.grad, w2._swr_hooked = torch.ones_like(w2), True            # (as a parameter of a gradient arena)
+    z, u = ops.norm_gate_residual(t["x"], t["y"], w_post=w2, w_pre=w2, scale=0.7)
+    torch.autograd.backward((z, u), (dz, du))
+    ref.check(w2.grad - 1, tuple(a + b + (2.0 ** -22 if i else 0) for i, (a, b) in enumerate(zip(want["dw_post"], want["dw_pre"]))), "arena")
+
+
 def test_captured_and_replayed():
     from scenario_wise_rec import ops
     t, dz, du = make(500, 200, BF16, PARTS, 3)

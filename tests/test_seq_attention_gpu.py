@@ -330,6 +330,86 @@ def test_gradients_against_differences():
         assert abs(got - want) <= (4 * h * h + 2.0 ** -12) * scale, (i, got, want, scale)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_given_scales(scale, dtype):
+    g, lens = gen(13), [150, 40]
+    q, k, v, dout = (randn(g, 190, 2, 32, dtype=dtype) for _ in range(4))
+    bias, tab = randn(g, 2, 8), table(8, 20, True)
+    got = run(q, k, v, dout, bias, cu_q=prefix(lens), max_q=150, buckets=tab, scale=scale)
+    compare(got, ref.attention(q, k, v, dout, lens, lens, [0, 150], [0, 150], True, scale, bias, tab))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_long_sequence_among_many_without_hints(dtype):
+    """The default launch is sized for four times the mean length: the long sequence is walked in rounds."""
+    g, lens = gen(14), [3] * 60 + [900] + [1] * 60
+    T = sum(lens)
+    q, k, v, dout = randn(g, T, 2, 32, dtype=dtype), randn(g, T, 1, 32, dtype=dtype), randn(g, T, 1, 32, dtype=dtype), randn(g, T, 2, 32, dtype=dtype)
+    bias, tab = randn(g, 2, 8), table(8, 20, True)
+    got = run(q, k, v, dout, bias, cu_q=prefix(lens), buckets=tab)
+    compare(got, ref.attention(q, k, v, dout, lens, lens, starts(lens), starts(lens), True, None, bias, tab))
+
+
+def test_largest_table_and_widest_group():
+    """The largest distance table the backward has room for, and many query heads on one key head; one more is refused."""
+    from scenario_wise_rec import _hip as H
+    from scenario_wise_rec import ops
+    g = gen(15)
+    for dtype in (F32, BF16):
+        q, k, v, dout = (randn(g, 70, 2, 128, dtype=dtype) for _ in range(4))
+        for causal in (True, False):
+            bias, tab = randn(g, 2, 256), table(256, 2048 if causal else 1024, causal)
+            got = run(q, k, v, dout, bias, cu_q=prefix([70]), causal=causal, buckets=tab)
+            compare(got, ref.attention(q, k, v, dout, [70], [70], [0], [0], causal, None, bias, tab))
+        q, dout = randn(g, 40, 93, 128, dtype=dtype), randn(g, 40, 93, 128, dtype=dtype)
+        k, v = randn(g, 40, 1, 128, dtype=dtype), randn(g, 40, 1, 128, dtype=dtype)
+        compare(run(q, k, v, dout, cu_q=prefix([40])), ref.attention(q, k, v, dout, [40], [40], [0], [0], True))
+    with pytest.raises(H.SwrError):
+        ops.seq_attention(q[:, :1].expand(40, 94, 128), k, v, prefix([40]))
+
+
+def test_rows_behind_the_last_sequence_are_zeros_in_a_large_buffer():
+    """A buffer of fixed size whose last rows no sequence uses, odd row sizes: every output row of them is zero."""
+    g = gen(16)
+    for H, D in ((3, 5), (2, 64)):
+        T = 60001
+        q, k, v, dout = (randn(g, T, H, D, dtype=BF16) for _ in range(4))
+        got = run(q, k, v, dout, cu_q=torch.tensor([7, 50, 107], dtype=torch.int32, device="cuda"), max_q=57)
+        for n, t in got.items():
+            assert not t[:7].any() and not t[107:].any() and t[7:107].any(), n
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^31 elements: its last sequence starts past 2^31."""
+    rows, H, D = (1 << 24) + 600, 1, 128
+    k, v = (torch.empty(rows, H, D, dtype=BF16, device="cuda") for _ in range(2))
+    g = gen(17)
+    first = (1 << 24) + 100
+    k[first:], v[first:] = randn(g, 500, H, D, dtype=BF16), randn(g, 500, H, D, dtype=BF16)
+    q, dout = randn(g, 40, 2, D, dtype=BF16), randn(g, 40, 2, D, dtype=BF16)
+    cu_k = torch.tensor([first, first + 500], dtype=torch.int32, device="cuda")
+    for new in (1, 40):
+        got = run(q[:new], k, v, dout[:new], grads=False, cu_q=prefix([new]), cu_k=cu_k, max_q=new, max_k=500)
+        compare(got, ref.attention(q[:new], k[first:], v[first:], dout[:new], [new], [500], [0], [0], True, train=False))
+
+
+def test_saved_tensors_may_move_and_the_graph_may_be_walked_twice():
+    """Saved tensors kept on the host between the passes; a second backward over the same graph; an expanded output gradient."""
+    from scenario_wise_rec import ops
+    g = gen(18)
+    for dtype in (F32, BF16):
+        leaves = [randn(g, 50, 2, 32, dtype=dtype).requires_grad_(True) for _ in range(3)]
+        out = ops.seq_attention(*leaves, prefix([50]))
+        base = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+        again = torch.autograd.grad(out.sum(), leaves)
+        with torch.autograd.graph.save_on_cpu():
+            out = ops.seq_attention(*leaves, prefix([50]))
+        moved = torch.autograd.grad(out.sum(), leaves)
+        for a, b, c in zip(base, again, moved):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_empty_inputs():
     from scenario_wise_rec import ops
     for tq, tk in ((0, 0), (0, 8), (8, 0)):

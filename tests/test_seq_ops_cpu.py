@@ -33,7 +33,7 @@ def test_struct_layouts_and_limits_match_the_header():
 
 
 @pytest.mark.parametrize("n,far,causal", [(2, 2, True), (3, 9, True), (16, 64, True), (32, 128, True), (32, 128, False), (4, 3, False),
-                                          (33, 1000, True), (256, 4000, True), (8, 2000, False)])
+                                          (33, 1000, True), (256, 2000, True), (8, 1000, False)])
 def test_bucket_table(n, far, causal):
     from scenario_wise_rec import ops
     t = ops.seq_buckets(n, far, causal, device="cpu")
@@ -53,7 +53,7 @@ def test_bucket_table(n, far, causal):
 
 def test_bucket_table_refusals():
     from scenario_wise_rec import ops
-    for args in ((1, 10, True), (0, 10, True), (7, 10, False), (2, 10, False), (300, 1000, True), (32, 16, True), (32, 5000, True), (32, 2100, False)):
+    for args in ((1, 10, True), (0, 10, True), (7, 10, False), (2, 10, False), (300, 1000, True), (32, 16, True), (32, 5000, True), (32, 1100, False)):
         with pytest.raises(ValueError):
             ops.seq_buckets(*args, device="cpu")
 
@@ -81,7 +81,7 @@ def test_attention_entry_refuses():
                      (-2, dict(dtype=H.F16)), (-2, dict(dtype=0)), (-3, dict(out=4104)), (-5, dict(D=129)), (-5, dict(Hk=3)),
                      (-5, dict(Tq=1 << 31)), (-5, dict(n_dist=8, n_buckets=4, bias=4096, buckets=4096, causal=0)),
                      (-5, dict(n_dist=5000, n_buckets=4, bias=4096, buckets=4096)),
-                     (-5, dict(n_dist=4097, n_buckets=4, bias=4096, buckets=4096, Hq=6)),
+                     (-5, dict(n_dist=2049, n_buckets=4, bias=4096, buckets=4096, Hq=12)), (-5, dict(Hq=200)), (-5, dict(B=1 << 30)),
                      (-5, dict(n_dist=9, n_buckets=257, bias=4096, buckets=4096))]:
         a = attention_args(**kw)
         assert call(a) == want, kw
