@@ -321,8 +321,10 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
         const int steps = n_r * a.G;
         SaStage<NP, DP, RT, NT, FAST> sQ, sD;
         float ld_l = 0.f, ld_d = 0.f;
-        auto fetch = [&](int step, int buf) {
-            const int h = hk * a.G + step / n_r, q0 = (r_begin + step % n_r) * RT;
+        int next_g = 0, next_r = 0;                    // head of the group and row tile of the step to fetch next
+        auto fetch = [&](int buf) {
+            const int h = hk * a.G + next_g, q0 = (r_begin + next_r) * RT;
+            if (++next_r == n_r) { next_r = 0; ++next_g; }
             if (Cfg::DMA) {
                 const sa_lds to = (sa_lds)smem + buf * 2 * TILE;
                 SaDma<DP, RT, NT>::copy(to, a.q, sq.q0, q0, sq.lq, a.q_row, static_cast<int64_t>(h) * a.q_head, a.D, nullptr);
@@ -349,19 +351,21 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                     sv.store(vt);
                 }
             }
-            if (!Cfg::LATE) fetch(0, 0);
+            if (!Cfg::LATE) fetch(0);
         }
         const SaArgs kv = sa_again();
         SaRows<NP, DP, FAST, Cfg::LATE> K, V;
         K.load(kv->k, row * kv->k_row + hk * kv->k_head, live, kv->D, kv->vk, lane);
         if (!Cfg::VL) V.load(kv->v, row * kv->v_row + hk * kv->v_head, live, kv->D, kv->vv, lane);
         if (tile == within) sa_bias_rows<NT>(a, hk * a.G, a.G, tables);
+        int g = 0, r = 0;
         for (int step = 0; step < steps; ++step) {
-            const int q0 = (r_begin + step % n_r) * RT, buf = Cfg::DMA ? step & 1 : 0;
+            const int q0 = (r_begin + r) * RT, buf = Cfg::DMA ? step & 1 : 0;
             const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
             float *lse_s = rows0 + buf * 2 * RT, *delta_s = lse_s + RT;
-            const float* bt = tables + (step / n_r) * a.row;
-            if (Cfg::LATE) fetch(step, 0);
+            const float* bt = tables + g * a.row;
+            if (++r == n_r) { r = 0; ++g; }
+            if (Cfg::LATE) fetch(0);
             if (!Cfg::DMA) {
                 if (step > 0) __syncthreads();
                 sQ.store(qt);
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
             if (threadIdx.x < RT) { lse_s[threadIdx.x] = ld_l; delta_s[threadIdx.x] = ld_d; }
             if (Cfg::DMA) sa_dma_wait();
             __syncthreads();
-            if (!Cfg::LATE && step + 1 < steps) fetch(step + 1, buf ^ 1);
+            if (!Cfg::LATE && step + 1 < steps) fetch(buf ^ 1);
             if (wfirst > wlast) continue;
 #pragma unroll 1
             for (int rb = 0; rb < RB; ++rb) {

@@ -69,17 +69,17 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             if (a.buckets[i] < 0 || a.buckets[i] >= a.n_buckets) atomicOr(a.err_flag, SWR_FLAG_INDEX_OOR);
     }
 
-    const int64_t ncol = static_cast<int64_t>(sq.q_span) * a.pack;
+    const int ncol = sq.q_span * a.pack;       // (below 2^31: the host packs heads only where all rows' columns are)
     const int64_t tile0 = a.tiles - 1 - within / ng;
     for (int64_t tile = tile0; tile * QT < ncol; tile += a.tiles) {
-        const int64_t col0 = tile * QT + wave * 32, col = col0 + (lane & 31);
-        const int tok = static_cast<int>(min(col, ncol) / a.pack), hsub = static_cast<int>(col % a.pack), h = h0 + hsub;
+        const int col0 = static_cast<int>(tile * QT) + wave * 32, col = col0 + (lane & 31);
+        const int tok = min(col, ncol) / a.pack, hsub = col % a.pack, h = h0 + hsub;
         const bool exists = col < ncol, live = exists && tok < sq.lq;
         const int qpos = tok + sq.shift;
         // the wave's and the workgroup's token range; keys any of them may read
-        const int wfirst = static_cast<int>(min(col0, ncol) / a.pack), wlast = static_cast<int>(min(static_cast<int64_t>(sq.lq), (min(col0 + 31, ncol - 1)) / a.pack + 1)) - 1;
-        const int bfirst = static_cast<int>(tile * QT / a.pack);
-        const int blast = static_cast<int>(min(static_cast<int64_t>(sq.lq), min(tile * QT + QT - 1, ncol - 1) / a.pack + 1)) - 1;
+        const int wfirst = min(col0, ncol) / a.pack, wlast = min(sq.lq, min(col0 + 31, ncol - 1) / a.pack + 1) - 1;
+        const int bfirst = static_cast<int>(tile * QT) / a.pack;
+        const int blast = min(sq.lq, min(static_cast<int>(tile * QT) + QT - 1, ncol - 1) / a.pack + 1) - 1;
         int kend = a.causal ? min(sq.lk, blast + sq.shift + 1) : sq.lk;
         if (bfirst >= sq.lq || kend < 0) kend = 0;
         const int ntile = (kend + KT - 1) / KT;
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256) void seq_attention_join_kernel(const SaK a) {
 int sa_check(const swr_seq_attention_args* p, bool backward) {
     SWR_REQUIRE(p, SWR_ERR_ARG);
     SWR_REQUIRE(p->B >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->max_q >= 0 && p->max_k >= 0, SWR_ERR_ARG);
-    SWR_REQUIRE(p->Tq < (1ll << 31) && p->Tk < (1ll << 31), SWR_ERR_UNSUPPORTED);
+    SWR_REQUIRE(p->Tq < (1ll << 31) - 4096 && p->Tk < (1ll << 31) - 4096, SWR_ERR_UNSUPPORTED);
     SWR_REQUIRE(p->dtype == SWR_F32 || p->dtype == SWR_BF16, SWR_ERR_DTYPE);
     SWR_REQUIRE(p->D >= 1 && p->Hk >= 1 && p->Hq >= p->Hk, SWR_ERR_ARG);
     SWR_REQUIRE(p->D <= SWR_SEQ_MAX_DIM && p->Hq % p->Hk == 0, SWR_ERR_UNSUPPORTED);
@@ -368,7 +368,7 @@ unsigned sa_grid(SaK& a) {
 // reads the same keys, so the group's heads share the columns.  splits: workgroups are added along the keys until the 256 CUs hold
 // two each, as long as a range keeps two tiles.
 static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
-    a.pack = a.G > 1 && p->max_q < 128 ? a.G : 1;
+    a.pack = a.G > 1 && p->max_q < 128 && p->Tq * a.G < (1ll << 31) - 4096 ? a.G : 1;
     const int64_t cols = static_cast<int64_t>(p->max_q) * a.pack;
     nw = sa_waves(cols, a, p->dtype == SWR_F32);
     const int64_t tiles = std::max<int64_t>(1, (cols + nw * 32 - 1) / (nw * 32));
