@@ -2876,6 +2876,8 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
     if bias is not None:
         if bias.dtype != torch.float32 or bias.dim() != 2 or bias.shape[0] != Hq or not 1 <= bias.shape[1] <= H.SEQ_MAX_BUCKETS:
             raise ValueError(f"seq_attention: bias must be float32 [{Hq}, n_buckets <= {H.SEQ_MAX_BUCKETS}], got {bias.dtype} {tuple(bias.shape)}")
+        if bias.device != q.device:
+            raise H.SwrError(f"seq_attention: bias is on {bias.device}, the queries on {q.device}")
         buckets = _index_vector(buckets, "buckets", buckets.numel(), q.device)
         if not 1 <= buckets.numel() <= H.SEQ_MAX_DIST or (not causal and buckets.numel() % 2 == 0):
             raise ValueError(f"seq_attention: {buckets.numel()} bucket entries (at most {H.SEQ_MAX_DIST}, odd when not causal)")

@@ -99,6 +99,19 @@ def test_attention_entry_refuses():
     assert bwd(a, 4096, lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a)) - 1) == -6
 
 
+def test_attention_refuses_a_bias_elsewhere(monkeypatch):
+    """A bias (or its buckets) on another device than the queries is refused before any pointer is taken."""
+    from scenario_wise_rec import _hip as H, ops
+    monkeypatch.setattr(H, "require_device", lambda *t: None)
+    q = torch.zeros(4, 2, 8, device="meta")
+    cu = torch.zeros(2, dtype=torch.int32, device="meta")
+    table = ops.seq_buckets(4, 8, device="cpu")
+    with pytest.raises(H.SwrError, match="bias is on cpu"):
+        ops.seq_attention(q, q, q, cu, bias=torch.zeros(2, 4), buckets=table.to("meta"))
+    with pytest.raises(H.SwrError, match="buckets is on cpu"):
+        ops.seq_attention(q, q, q, cu, bias=torch.zeros(2, 4, device="meta"), buckets=table)
+
+
 def test_norm_entry_refuses():
     from scenario_wise_rec import _hip as H
     lib = H.lib
