@@ -151,14 +151,25 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 if (wfirst > wlast || k0 >= sq.lk || (a.causal && k0 > wlast + sq.shift)) continue;      // (whole waves)
                 ln.fresh();
                 f32x16 S = sa_zero16(), dP = sa_zero16();
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                    bf16x8 A[NP];
-                    ln.rows(kt, kb, s, A);
-                    S = sa_mma(A, Q[s], S);
-                    ln.rows(vt, kb, s, A);
-                    dP = sa_mma(A, dO[s], dP);
+                {
+                    bf16x8 A[2][2][NP];
+                    sa_ahead<DP / 16, true>(
+                        [&](int buf, int s) {
+                            ln.rows(kt, kb, s, A[buf][0]);
+                            ln.rows(vt, kb, s, A[buf][1]);
+                        },
+                        [&](int buf, int s) {
+                            S = sa_mma(A[buf][0], Q[s], S);
+                            dP = sa_mma(A[buf][1], dO[s], dP);
+                        });
                 }
+                // (the second product's first operands come in under the exponentials)
+                bf16x8 T[2][DP / 32][NP];
+                auto cols = [&](int buf, int ks) {
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) ln.cols(kt, kb * 2 + ks, db, T[buf][db]);
+                };
+                cols(0, 0);
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
                 const SaSpan sp = sa_span(a, near_d, far_d);
                 if (sp.apart) {
@@ -210,20 +221,18 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                         else acc[a.causal ? dist : dist + a.reach] += sum;
                     }
                 }
+                bf16x8 P[2][NP];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     float f[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) f[j] = S[8 * ks + j];
-                    bf16x8 P[NP];
-                    sa_planes_f(f, P);
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) {
-                        bf16x8 A[NP];
-                        ln.cols(kt, kb * 2 + ks, db, A);
-                        dQ[db] = sa_mma(A, P, dQ[db]);
-                    }
+                    sa_planes_f(f, P[ks]);
                 }
+                sa_ahead<2, false>(cols, [&](int buf, int ks) {
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) dQ[db] = sa_mma(T[buf][db], P[ks], dQ[db]);
+                });
             }
         }
         if (exists) {
@@ -382,17 +391,31 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 if (r0 >= sq.lq || (a.causal && rlast + sq.shift < wfirst)) continue;
                 ln.fresh();
                 f32x16 S = sa_zero16(), dP = sa_zero16();
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                    bf16x8 A[NP], B[NP];
-                    ln.rows(qt, rb, s, A);
-                    K.get(s, B);
-                    S = sa_mma(A, B, S);
-                    ln.rows(dt, rb, s, A);
-                    if constexpr (Cfg::VL) ln.rows(vt + wave * (32 * DP * 2), 0, s, B);
-                    else V.get(s, B);
-                    dP = sa_mma(A, B, dP);
+                {
+                    bf16x8 A[2][2][NP];
+                    sa_ahead<DP / 16, true>(
+                        [&](int buf, int s) {
+                            ln.rows(qt, rb, s, A[buf][0]);
+                            ln.rows(dt, rb, s, A[buf][1]);
+                        },
+                        [&](int buf, int s) {
+                            bf16x8 B[NP];
+                            K.get(s, B);
+                            S = sa_mma(A[buf][0], B, S);
+                            if constexpr (Cfg::VL) ln.rows(vt + wave * (32 * DP * 2), 0, s, B);
+                            else V.get(s, B);
+                            dP = sa_mma(A[buf][1], B, dP);
+                        });
                 }
+                // dv and dk take the rows in two halves each: group 2 ks + (0 dv, 1 dk).  (The first operands come in under the exponentials,
+                // where the registers hold them)
+                constexpr bool FULL = NP == 1 && DP == 128 && NW == 4;
+                bf16x8 T[2][DP / 32][NP];
+                auto cols = [&](int buf, int i) {
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) ln.cols(i & 1 ? qt : dt, rb * 2 + (i >> 1), db, T[buf][db]);
+                };
+                if (!FULL) cols(0, 0);
                 // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
                 // behind the last query have lse = +inf, p = 0)
                 const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
@@ -409,27 +432,18 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
+                sa_ahead<4, FULL>(cols, [&](int buf, int i) {
                     float f[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = S[8 * ks + j];
-                    bf16x8 P[NP], A[NP];
+                    for (int j = 0; j < 8; ++j) f[j] = i & 1 ? dP[8 * (i >> 1) + j] : S[8 * (i >> 1) + j];
+                    bf16x8 P[NP];
                     sa_planes_f(f, P);
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
-                        ln.cols(dt, rb * 2 + ks, db, A);
-                        dV[db] = sa_mma(A, P, dV[db]);
+                        if (i & 1) dK[db] = sa_mma(T[buf][db], P, dK[db]);
+                        else dV[db] = sa_mma(T[buf][db], P, dV[db]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = dP[8 * ks + j];
-                    sa_planes_f(f, P);
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) {
-                        ln.cols(qt, rb * 2 + ks, db, A);
-                        dK[db] = sa_mma(A, P, dK[db]);
-                    }
-                }
+                });
             }
         }
         if (exists) {

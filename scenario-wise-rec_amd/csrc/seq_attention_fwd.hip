@@ -136,15 +136,21 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             ln.fresh();
             f32x16 S[KB];
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                S[kb] = sa_zero16();
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                    bf16x8 A[NP];
-                    ln.rows(kt, kb, s, A);
-                    S[kb] = sa_mma(A, Q[s], S[kb]);
-                }
+            for (int kb = 0; kb < KB; ++kb) S[kb] = sa_zero16();
+            {
+                constexpr int NS = DP / 16;
+                bf16x8 A[2][NP];
+                sa_ahead<KB * NS, true>([&](int b, int i) { ln.rows(kt, i / NS, i % NS, A[b]); },
+                                        [&](int b, int i) { S[i / NS] = sa_mma(A[b], Q[i % NS], S[i / NS]); });
             }
+            // (the second product's first operands come in under the exponentials, where the registers hold them)
+            constexpr bool FULL = NP == 3 && DP == 64 && NW == 4;
+            bf16x8 T[2][DP / 32][NP];
+            auto cols = [&](int b, int ks) {
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) ln.cols(vt, ks, db, T[b][db]);
+            };
+            if (!FULL) cols(0, 0);
             // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
             // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
             const float* bh = bt + hsub * a.row;
@@ -209,20 +215,15 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 }
                 l += sum;
             }
-#pragma unroll
-            for (int ks = 0; ks < KT / 16; ++ks) {
+            sa_ahead<KT / 16, FULL>(cols, [&](int b, int ks) {
                 float pf[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pf[j] = S[ks >> 1][8 * (ks & 1) + j];
                 bf16x8 P[TRAIN ? 2 : NP];
                 sa_planes_f(pf, P);
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    bf16x8 A[NP];
-                    ln.cols(vt, ks, db, A);
-                    O[db] = sa_mma(A, P, O[db]);
-                }
-            }
+                for (int db = 0; db < DP / 32; ++db) O[db] = sa_mma(T[b][db], P, O[db]);
+            });
         }
         l += __shfl_xor(l, 32);
         if (!live) {                           // a column without a query went through the products as a row of zeros
