@@ -267,18 +267,17 @@ struct SaLane {
         }
     }
 };
-// N groups of left operands one ahead of their products: load(buffer, i) brings group i from LDS into registers, mul(buffer, i) uses it.
-// The fences keep the order -- left to itself the compiler puts a read right in front of its product and every matrix instruction
-// waits for LDS.  Without FIRST the first group has been loaded before.  Measured (the same products without it): training steps of 24
-// packed sequences up to 2 048, heads of 64, bf16, 0.92 / 1.00 ms, of 4 sequences up to 4 096, heads of 128, 1.25 / 1.32 ms; prompts up
-// to 8 192 2.33 / 2.44 ms; 64 fp32 sequences up to 600 both ways 0.150 / 0.155 ms.  Two or four groups together: the same times.
+// N groups of left operands one ahead of their products: load(buffer, i) brings group i from LDS into registers, mul(buffer, i) uses it
+// -- a read right in front of its product makes the matrix instruction wait for LDS.  Without FIRST the first group has been loaded
+// before.  Measured (without it): training steps of 24 packed sequences up to 2 048, heads of 64, bf16, 0.91 / 1.00 ms, of 4 sequences up
+// to 4 096, heads of 128, 1.22 / 1.32 ms; prompts up to 8 192 2.29 / 2.44 ms; 64 fp32 sequences up to 600 both ways 0.148 / 0.155 ms.
+// Two or four groups together take the same times, a fence between read and product 1 % more.
 template <int N, bool FIRST, class Load, class Mul>
 __device__ __forceinline__ void sa_ahead(Load load, Mul mul) {
     if (FIRST) load(0, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (i + 1 < N) load((i + 1) & 1, i + 1);
-        __builtin_amdgcn_sched_barrier(0);
         mul(i & 1, i);
     }
 }

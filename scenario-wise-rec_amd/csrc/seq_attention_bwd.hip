@@ -407,15 +407,13 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                             dP = sa_mma(A[buf][1], B, dP);
                         });
                 }
-                // dv and dk take the rows in two halves each: group 2 ks + (0 dv, 1 dk).  (The first operands come in under the exponentials,
-                // where the registers hold them)
-                constexpr bool FULL = NP == 1 && DP == 128 && NW == 4;
+                // dv and dk take the rows in two halves each: group 2 ks + (0 dv, 1 dk); the first operands come in under the exponentials
                 bf16x8 T[2][DP / 32][NP];
                 auto cols = [&](int buf, int i) {
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) ln.cols(i & 1 ? qt : dt, rb * 2 + (i >> 1), db, T[buf][db]);
                 };
-                if (!FULL) cols(0, 0);
+                cols(0, 0);
                 // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
                 // behind the last query have lse = +inf, p = 0)
                 const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
@@ -432,7 +430,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
-                sa_ahead<4, FULL>(cols, [&](int buf, int i) {
+                sa_ahead<4, false>(cols, [&](int buf, int i) {
                     float f[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) f[j] = i & 1 ? dP[8 * (i >> 1) + j] : S[8 * (i >> 1) + j];

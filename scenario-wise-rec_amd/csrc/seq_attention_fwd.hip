@@ -143,14 +143,13 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 sa_ahead<KB * NS, true>([&](int b, int i) { ln.rows(kt, i / NS, i % NS, A[b]); },
                                         [&](int b, int i) { S[i / NS] = sa_mma(A[b], Q[i % NS], S[i / NS]); });
             }
-            // (the second product's first operands come in under the exponentials, where the registers hold them)
-            constexpr bool FULL = NP == 3 && DP == 64 && NW == 4;
+            // (the second product's first operands come in under the exponentials)
             bf16x8 T[2][DP / 32][NP];
             auto cols = [&](int b, int ks) {
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) ln.cols(vt, ks, db, T[b][db]);
             };
-            if (!FULL) cols(0, 0);
+            cols(0, 0);
             // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
             // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
             const float* bh = bt + hsub * a.row;
@@ -215,7 +214,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 }
                 l += sum;
             }
-            sa_ahead<KT / 16, FULL>(cols, [&](int b, int ks) {
+            sa_ahead<KT / 16, false>(cols, [&](int b, int ks) {
                 float pf[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pf[j] = S[ks >> 1][8 * (ks & 1) + j];
