@@ -26,8 +26,8 @@ __device__ __forceinline__ Bf3 split3(float x) {
         L[idx] = s3_.l;                    \
     } while (0)
 
-// Two values at a time: v_cvt_pk_bf16_f32 rounds both, v_pk_add_f32 takes both remainders -- 4.5 VALU per value instead
-// of 7 (the split is the VALU work that sits in front of every MFMA group); bit-identical to split3().
+// Two values at a time: v_cvt_pk_bf16_f32 rounds both (the remainders are taken one by one, the build has no packed fp32 arithmetic):
+// fewer VALU per value than one at a time (the split is the VALU work that sits in front of every MFMA group); bit-identical to split3().
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 #ifdef SWR_SPLIT_SCALAR
