@@ -381,6 +381,11 @@ __device__ __forceinline__ float sa_bias2(float b) {
     const float x = b * SA_LOG2E;
     return (__builtin_isinf(x) && !__builtin_isinf(b)) ? copysignf(3.402823466e38f, x) : x;
 }
+// Scores are fp32 values, s = S c + bias rounded once: a large bias absorbs digits of the products, all of them at the type's lowest
+// value.  Every block of a row has to round alike, or the same keys weigh differently in blocks of one bias (whose raw products would
+// enter beside bias - maximum, and overflow) and in blocks that touch the table.  Up to 2^10 the digits lost are below 2^-14 of a score,
+// and the one fma of raw products, bias and maximum stays.  (-inf absorbs everything in either form.)
+__device__ __forceinline__ bool sa_wide(float add) { return fabsf(add) > 1024.f && add != -INFINITY; }
 __device__ __forceinline__ int sa_bucket(const SaK& a, int i) { return max(0, min(a.buckets[i], a.n_buckets - 1)); }
 // rows of heads h .. h + heads - 1.  A value is two loads deep (bucket, bias) and a single token's whole work is a few loads deep: every
 // thread has the buckets of several entries in flight, then their values (one wave, 193 entries, one after the other: the query pass of

@@ -151,7 +151,8 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
             };
             cols(0, 0);
             // A block's exponents are x = S mul + add: a block of one bias keeps the raw products (mul = c, folded into one fma with the
-            // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0).
+            // row's maximum below), one that touches the table or hides keys is written out (mul = 1, add = 0), and so is one whose bias
+            // absorbs digits of the products (sa_wide).
             const float* bh = bt + hsub * a.row;
             float mul[KB], add[KB], mx = -INFINITY;
 #pragma unroll
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 const bool cut = !a.causal && kf + 32 > sq.lk;                    // (causal: keys behind the last are masked by distance)
                 mul[kb] = a.c;
                 add[kb] = sp.apart && a.row ? bh[sp.entry] : 0.f;
-                if (!sp.apart || cut || a.key_mask || a.c < 0.f) {
+                if (!sp.apart || cut || a.key_mask || a.c < 0.f || __any(sa_wide(add[kb]))) {
                     if (sp.apart) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + add[kb];
