@@ -807,7 +807,8 @@ int swr_block_select_bwd(const float* dout, int64_t ldo, const void* domain, int
  * counterpart: the reference pools a history by sum / mean / concat, basic/layers.py:174-228).
  *   s_ij = scale q_i . k_j + bias[h, buckets[entry(i + lk - lq - j)]]      i < lq, j < lk of one sequence, h = query head
  *   out_i = sum_j softmax_j(s_ij) v_j over the allowed j: key_mask[j] != 0 and, causal, j <= i + lk - lq
- * A row with no allowed key is zeros, and so are its gradients.  Query head h reads key head h / (Hq / Hk).  Values in use are
+ * s is held in fp32: a bias of large magnitude absorbs digits of the product (all of them at the type's lowest value: keys that carry it
+ * alike weigh alike).  A row with no allowed key is zeros, and so are its gradients.  Query head h reads key head h / (Hq / Hk).  Values in use are
  * expected to be finite: what is hidden by key_mask or lies beyond the lengths may be anything, but a NaN or infinity behind the
  * causal border enters products with zeros and may spread to earlier rows of its sequence.
  * Sequence b: query rows cu_q[b] .. cu_q[b + 1], key rows cu_k[b] .. cu_k[b + 1] (prefix sums, int32, B + 1 entries); q_len / k_len
@@ -833,7 +834,9 @@ typedef struct {
     const void* k; int64_t k_row, k_head;
     const void* v; int64_t v_row, v_head;
     void* out;
-    float* lse;                        /* [Hq, Tq] log2 of the softmax sums, +inf for an empty row; NULL in a forward without a backward */
+    float* lse;                        /* [2, Hq, Tq]: p = 2^(s log2 e - first) second -- log2 of the softmax sum (+inf for an empty row) and 1,
+                                          or, where that would be rounded away, the row's exponent and 1 / sum.  NULL in a forward
+                                          without a backward */
     float* out32;                      /* SWR_BF16 with lse: out before its rounding, [Tq, Hq, D], kept for the backward (its row products
                                           do . o have to agree with the score gradients' fp32 sums); SWR_F32: not used */
     const int32_t* cu_q; const int32_t* cu_k; const int32_t* q_len; const int32_t* k_len;

@@ -32,7 +32,7 @@ struct SaK {
     int vq, vk, vv, vo, vdo;               // elements per load of q, k, v, out, dout rows: 8, 4 or 1
     bool fast;                             // all of them 8, row strides below 2^23 elements (64 rows within 32-bit byte offsets)
     const void *q, *k, *v; int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-    void* out; float* lse; float* out32;
+    void* out; float* lse; float* out32;   // lse: [2][Hq][Tq] (sa_keep_sum)
     const int32_t *cu_q, *cu_k, *q_len, *k_len;
     const uint8_t* key_mask;
     const float* bias; const int32_t* buckets;
@@ -141,6 +141,8 @@ __device__ __forceinline__ int sa_here(int x) {
     asm volatile("" : "+v"(x));
     return x;
 }
+// the same for a uniform value (a flag: without it the loop it is constant in is compiled once for either value, with more registers)
+__device__ __forceinline__ void sa_scalar_here(int& x) { asm volatile("" : "+s"(x)); }
 // The kernel's arguments read again where they are used: what only the start and the end of a tile need does not sit in scalar
 // registers through its inner loop.
 typedef const __attribute__((address_space(4))) SaK* SaArgs;
@@ -326,6 +328,17 @@ struct SaRows<NP, DP, FAST, true> {
     }
 };
 
+// What the forward keeps of a row's softmax, in two parts: p = 2^(x - first) second.  first = m + log2 l and second = 1 where m is small
+// enough that the sum keeps log2 l to 2^-18; beside a large m (large scores, a large bias on every key of the row) it would be rounded away
+// and p would no longer sum to one (to the number of keys at the type's lowest value): there first = m, which x is near, second = 1 / l.
+// A row without a key: +inf, 1.  The backward reads second parts only where a row's first says that there may be one (sa_parts).
+__device__ __forceinline__ bool sa_parts(float first) { return fabsf(first) > 64.f && first != INFINITY; }
+__device__ __forceinline__ void sa_keep_sum(float* lse, int64_t at, int64_t rows, float m, float l) {
+    const bool two = l != 0.f && sa_parts(m);
+    lse[at] = l == 0.f ? INFINITY : (two ? m : m + __builtin_amdgcn_logf(l));
+    lse[rows + at] = two ? 1.f / l : 1.f;
+}
+
 // 4 consecutive result columns d .. d + 3 of a row at `p` (row of D elements)
 template <int NP>
 __device__ __forceinline__ void sa_store4(void* base, int64_t row_off, int d, int D, const float* x) {
@@ -425,6 +438,22 @@ __device__ __forceinline__ SaSpan sa_span(const SaK& a, int near_d, int far_d) {
     s.entry = hi ? (a.causal ? a.reach : 2 * a.reach) + SA_PAD : SA_PAD;
     return s;
 }
+// whether the bias beyond the reach (either side) is sa_wide for one of this lane's of the heads h .. h + heads - 1
+__device__ __forceinline__ bool sa_wide_ends(const SaK& a, int h, int heads, int lane) {
+    bool w = false;
+    if (a.n_dist) {
+        const int near_b = sa_bucket(a, 0), far_b = sa_bucket(a, a.n_dist - 1);
+        for (int i = lane; i < heads; i += 64) {
+            const float* b = a.bias + (h + i) * a.n_buckets;
+            w |= sa_wide(sa_bias2(b[far_b])) || (!a.causal && sa_wide(sa_bias2(b[near_b])));
+        }
+    }
+    return w;
+}
+// the first of 28 entries that hold a block's one value (the padded ends; SA_FLAT zeros where there is no row): the backward's form for it in
+// a row whose lse is in two parts
+#define SA_FLAT 28
+__device__ __forceinline__ int sa_flat_entry(const SaK& a, SaSpan s) { return a.row == 0 || (s.entry == SA_PAD && a.reach) ? 0 : s.entry; }
 // entry of distance d
 __device__ __forceinline__ int sa_entry(const SaK& a, int d) { return d + SA_PAD + (a.causal ? 0 : a.reach); }
 // hidden key of result row i (km: the block's flags from row 4 hi on, 4-byte aligned)

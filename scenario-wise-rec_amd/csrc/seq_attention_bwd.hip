@@ -1,6 +1,6 @@
 // Attention over packed sequences, backward (seq_attention_fwd.hip has the forward and its definitions).
 //
-//   p_ij = 2^(x_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   p_ij = 2^(x_ij - lse_i) (times a second part where lse is large, sa_keep_sum),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,   dbias[h, t] = sum of ds over bucket t
 //
 // Two passes that recompute the scores, so that every sum has one owner and a fixed order (no atomics): a workgroup of query columns
@@ -30,7 +30,7 @@ struct SaDq {
     static constexpr bool DMA = FAST && NP == 1;
     static constexpr int KT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr int TILE = NP * KT * DP * 2;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (a.row + (a.bias_part ? NW * (SA_SKEW + a.n_dist) + a.n_dist + 2 * a.n_buckets : 0)) * 4; }
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + KT) + (max(a.row, SA_FLAT) + (a.bias_part ? NW * (SA_SKEW + a.n_dist) + a.n_dist + 2 * a.n_buckets : 0)) * 4; }
 };
 template <int NP, int DP, int NW, bool FAST>
 struct SaDkv {
@@ -38,7 +38,7 @@ struct SaDkv {
     static constexpr int RT = (NW == 1 || DP == 128) ? 32 : 64, NBUF = DMA ? 2 : 1;
     static constexpr bool VL = NP == 1 && DP == 128;           // the wave's values stay in LDS: with them in registers one wave fits a SIMD
     static constexpr int TILE = NP * RT * DP * 2, VTILE = VL ? NW * 32 * DP * 2 : 0;
-    static int lds(const SaK& a) { return NBUF * (2 * TILE + 2 * RT * 4) + VTILE + a.G * a.row * 4; }
+    static int lds(const SaK& a) { return NBUF * (2 * TILE + 2 * RT * 4) + VTILE + max(a.G * a.row, SA_FLAT) * 4; }
 };
 
 template <int NP, int DP, int NW, bool FAST>
@@ -116,8 +116,10 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
         }
         delta += __shfl_xor(delta, 32);
         const float lse = live ? n->lse[at] : INFINITY;
+        const bool parts = __any(sa_parts(lse));       // (then the scores are written out as the forward rounded them, also under one bias)
         if (tile == tile0) {
             sa_bias_rows<NT>(a, h, 1, bt);
+            if (a.row == 0 && threadIdx.x < SA_FLAT) bt[threadIdx.x] = 0.f;
             if (a.bias_part) {
                 for (int i = lane; i < SA_SKEW / 4; i += 64) reinterpret_cast<float4*>(skew)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int i = lane; i < a.n_dist; i += 64) acc[i] = 0.f;
@@ -172,16 +174,22 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 cols(0, 0);
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
                 const SaSpan sp = sa_span(a, near_d, far_d);
-                if (sp.apart) {
+                if (sp.apart && !parts) {
                     const float add = (a.row ? bt[sp.entry] : 0.f) - lse;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + add) * (dP[i] - delta);
                 } else {
-                    const float* be = bt + sa_entry(a, qpos - k0 - 4 * hi - 27);
+                    const float* be = bt + (sp.apart ? sa_flat_entry(a, sp) : sa_entry(a, qpos - k0 - 4 * hi - 27));
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float p = __builtin_amdgcn_exp2f((S[i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)]) - lse);
                         S[i] = p * (dP[i] - delta);
+                    }
+                    if (parts) {
+                        const SaArgs n = sa_again();
+                        const float part = n->lse[static_cast<int64_t>(n->Hq + h) * n->Tq + row];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) S[i] *= part;
                     }
                 }
                 if (!a.causal && k0 + 32 > sq.lk) {
@@ -366,13 +374,17 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
         SaRows<NP, DP, FAST, Cfg::LATE> K, V;
         K.load(kv->k, row * kv->k_row + hk * kv->k_head, live, kv->D, kv->vk, lane);
         if (!Cfg::VL) V.load(kv->v, row * kv->v_row + hk * kv->v_head, live, kv->D, kv->vv, lane);
-        if (tile == within) sa_bias_rows<NT>(a, hk * a.G, a.G, tables);
+        if (tile == within) {
+            sa_bias_rows<NT>(a, hk * a.G, a.G, tables);
+            if (a.row == 0 && threadIdx.x < SA_FLAT) tables[threadIdx.x] = 0.f;
+        }
         int g = 0, r = 0;
         for (int step = 0; step < steps; ++step) {
             const int q0 = (r_begin + r) * RT, buf = Cfg::DMA ? step & 1 : 0;
             const sa_lds qt = (sa_lds)smem + buf * 2 * TILE, dt = qt + TILE;
             float *lse_s = rows0 + buf * 2 * RT, *delta_s = lse_s + RT;
             const float* bt = tables + g * a.row;
+            const int h = hk * a.G + g;
             if (++r == n_r) { r = 0; ++g; }
             if (Cfg::LATE) fetch(0);
             if (!Cfg::DMA) {
@@ -407,6 +419,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                             dP = sa_mma(A[buf][1], B, dP);
                         });
                 }
+                const float first = lse_s[rb * 32 + (sa_here(lane) & 31)];
                 // dv and dk take the rows in two halves each: group 2 ks + (0 dv, 1 dk); the first operands come in under the exponentials
                 bf16x8 T[2][DP / 32][NP];
                 auto cols = [&](int buf, int i) {
@@ -417,16 +430,29 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
                 // (columns that are no key in use compute something finite or not: columns do not mix, theirs is not stored.  Rows
                 // behind the last query have lse = +inf, p = 0)
                 const SaSpan sp = sa_span(a, r0 + sq.shift - wlast, rlast + sq.shift - wfirst);
-                const float *lr = lse_s + rb * 32 + 4 * hi, *dr = delta_s + rb * 32 + 4 * hi;
-                if (sp.apart) {
+                const float *lr = lse_s + rb * 32 + ((sa_here(threadIdx.x) >> 3) & 4), *dr = lr + RT;
+                const bool parts = __any(sa_parts(first));             // (as in the query pass)
+                if (sp.apart && !parts) {
                     const float add = a.row ? bt[sp.entry] : 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + (add - lr[8 * (i >> 2) + (i & 3)]));
                 } else {
-                    const float* be = bt + sa_entry(a, r0 + 4 * hi + sq.shift - key);
+                    const int l = sa_here(threadIdx.x) & 63;
+                    const float* be = bt + (sp.apart ? sa_flat_entry(a, sp) : sa_entry(a, r0 + 4 * (l >> 5) + sq.shift - wfirst - (l & 31)));
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         S[i] = __builtin_amdgcn_exp2f((S[i] * a.c + be[8 * (i >> 2) + (i & 3)]) - lr[8 * (i >> 2) + (i & 3)]);
+                    if (parts) {
+                        const SaArgs n = sa_again();
+                        const float* second = n->lse + static_cast<int64_t>(n->Hq + h) * n->Tq + sq.q0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            // (one after the other: this rare path takes no registers from the others)
+                            float p = S[i] * second[min(r0 + ((sa_here(threadIdx.x) >> 3) & 4) + 8 * (i >> 2) + (i & 3), sq.lq - 1)];
+                            asm volatile("" : "+v"(p) : : "memory");
+                            S[i] = p;
+                        }
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - dr[8 * (i >> 2) + (i & 3)]);
@@ -445,7 +471,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DKV(NP, DP, NW, FAST)) void seq_a
             }
         }
         if (exists) {
-            const int64_t o = (row * a.Hk + hk) * a.D;
+            const int64_t o = ((sq.k0 + wfirst + (sa_here(threadIdx.x) & 31)) * a.Hk + hk) * a.D;       // (places made anew: no registers spill)
             const int hi4 = sa_here(4 * hi);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)

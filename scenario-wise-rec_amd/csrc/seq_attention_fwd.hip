@@ -4,7 +4,8 @@
 //
 // allowed: j < lk, key_mask[j], and j <= i + lk - lq when causal (the last query stands at the last key).  One pass over the keys with
 // the running maximum m and sum l of every row (both fp32, base-2 exponents: p = 2^(x - m), x = s log2 e); a row without an allowed
-// key keeps l = 0 and is written as zeros.  Saved for the backward: lse = m + log2 l (+inf for an empty row: every p becomes 0).
+// key keeps l = 0 and is written as zeros.  Saved for the backward: m + log2 l, in two parts where m is large (+inf for an empty row: every
+// p becomes 0).
 //
 // A workgroup holds NW x 32 columns = query rows (token-major, `pack` heads of a key head side by side), S^T = K Q^T and
 // O^T = V^T P^T (seq_attention.h); the keys and values of a tile are staged in LDS once for all its columns.  Few queries: the key
@@ -71,6 +72,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
 
     const int ncol = sq.q_span * a.pack;       // (below 2^31: the host packs heads only where all rows' columns are)
     const int64_t tile0 = a.tiles - 1 - within / ng;
+    int wide = 0;                              // the bias of blocks beyond the reach (either side) is sa_wide
     for (int64_t tile = tile0; tile * QT < ncol; tile += a.tiles) {
         const int col0 = static_cast<int>(tile * QT) + wave * 32, col = col0 + (lane & 31);
         const int tok = min(col, ncol) / a.pack, hsub = col % a.pack, h = h0 + hsub;
@@ -112,7 +114,11 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
         for (int db = 0; db < DP / 32; ++db) O[db] = sa_zero16();
         float m = -INFINITY, l = 0.f;
 
-        if (tile == tile0) sa_bias_rows<NT>(a, h0, a.pack, bt);
+        if (tile == tile0) {
+            const bool ends = sa_wide_ends(a, h0, a.pack, lane);       // (in flight beside the rows')
+            sa_bias_rows<NT>(a, h0, a.pack, bt);
+            wide = __builtin_amdgcn_readfirstlane(__any(ends));
+        }
         for (int t = t0; t < t1; ++t) {
             const int buf = Cfg::DMA ? (t - t0) & 1 : 0;
             const sa_lds kt = (sa_lds)smem + buf * 2 * TILE, vt = kt + TILE;
@@ -130,6 +136,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 __syncthreads();
             }
             if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+            sa_scalar_here(wide);
             const int k0 = t * KT;
             if (wfirst > wlast || (a.causal && k0 > wlast + sq.shift)) continue;
 
@@ -162,7 +169,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                 const bool cut = !a.causal && kf + 32 > sq.lk;                    // (causal: keys behind the last are masked by distance)
                 mul[kb] = a.c;
                 add[kb] = sp.apart && a.row ? bh[sp.entry] : 0.f;
-                if (!sp.apart || cut || a.key_mask || a.c < 0.f || __any(sa_wide(add[kb]))) {
+                if (!sp.apart || cut || a.key_mask || a.c < 0.f || wide) {
                     if (sp.apart) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) S[kb][i] = S[kb][i] * a.c + add[kb];
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES(NP, DP, NW)) void seq_attention_f
                         sa_store4<NP>(a.out, row, db * 32 + 2 * i + hi4, a.D, x);
                         if (TRAIN) sa_store4<3>(a.out32, row, db * 32 + 2 * i + hi4, a.D, x);
                     }
-                if (a.lse && hi == 0) a.lse[at] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+                if (a.lse && hi == 0) sa_keep_sum(a.lse, at, static_cast<int64_t>(a.Hq) * a.Tq, m, l);
             } else {
                 const int64_t pr = split * static_cast<int64_t>(a.Hq) * a.Tq + at;
                 if (hi == 0) { a.part[2 * pr] = m; a.part[2 * pr + 1] = l; }
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(256) void seq_attention_join_kernel(const SaK a) {
     const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     sa_store4<NP>(a.out, (t * a.Hq + h) * a.D, 4 * j, a.D, x);
     if (NP == 1 && a.out32) sa_store4<3>(a.out32, (t * a.Hq + h) * a.D, 4 * j, a.D, x);
-    if (a.lse && j == 0) a.lse[at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+    if (a.lse && j == 0) sa_keep_sum(a.lse, at, rows, M, L);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host

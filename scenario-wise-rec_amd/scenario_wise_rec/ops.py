@@ -2775,7 +2775,7 @@ class SeqAttention(Function):
     def launch(want, meta, q, k, v, bias, cu_q, cu_k, q_len, k_len, key_mask, buckets):
         """-> out, and what the backward needs besides: lse (None unless `want`), the unrounded rows."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
+        lse = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want else None
         out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want and q.dtype != torch.float32 else None
         a = _seq_args(meta, q, k, v, out, lse, out32, cu_q, cu_k, q_len, k_len, key_mask, bias, buckets)
         nbytes = lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a))

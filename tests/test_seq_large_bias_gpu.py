@@ -78,3 +78,141 @@ def test_far_keys_of_lowest_bias_beside_ordinary_ones(dtype):
         b = hidden.clone()
         b[:, -1] = far
         ref.check(ops.seq_attention(q, k, v, prefix(L), max_q=L, bias=b, buckets=one_each(n)), want, f"out {far}")
+
+
+# ---------------------------------------------------------------------------------------------------------------- gradients
+def one_head(q, k, v, dout, add, slot, n_buckets, causal, scale):
+    """-> {name: (value, allowed error)} of one head in 64 bits.  add [lq, lk]: the bias of every score; where it is 1e9 or more in
+    magnitude it absorbs the product, and where the row's products are zeros (q = 0) and its biases equal the scores are exact: neither
+    adds an error of the scores.  The other errors are counted as in _seq_reference."""
+    lq, lk, D = q.shape[0], k.shape[0], q.shape[1]
+    bf16, f = q.dtype == BF16, ref.f
+    u = 2.0 ** -8 if bf16 else 2.0 ** -24
+    r, rf = (u, 2.0 ** -16) if bf16 else (f(16), f(16))
+    Q, K, V, dO, add = (t.double() for t in (q, k, v, dout, add))
+    dist = (torch.arange(lq, device="cuda") + lk - lq)[:, None] - torch.arange(lk, device="cuda")[None]
+    ok = dist >= 0 if causal else torch.ones_like(dist, dtype=torch.bool)
+    mag = Q.abs() @ K.abs().t() * scale
+    s = torch.where(add.abs() >= 1e9, add, Q @ K.t() * scale + add)
+    exact = (add.abs() >= 1e9) | ((mag == 0) & (add == add[:, :1]))
+    es = torch.where(exact, 0., (f(D) + 4 * 2.0 ** -24) * (mag + add.abs()) + 2.0 ** -23 * s.abs())
+    p = torch.softmax(s.masked_fill(~ok, float("-inf")), 1)
+    es = torch.where(p > 0, es, 0.)                       # (keys that weigh nothing beside the row's others)
+    ep = (es + es.max(1, keepdim=True).values + 2.0 ** -20) * p
+    o = p @ V
+    eo = ep @ V.abs() + (rf + f(lk)) * (p @ V.abs())
+    dp, delta = dO @ V.t(), (dO * o).sum(1, keepdim=True)
+    size = dO.abs() @ V.abs().t() + (dO.abs() * o.abs()).sum(1, keepdim=True)
+    ed = (dO.abs() * (2.0 ** -24 * o.abs() + eo)).sum(1, keepdim=True) + f(D) * size
+    ds = p * (dp - delta)
+    eds = ep * (dp - delta).abs() + p * ed + 4 * 2.0 ** -24 * p * size
+    edsr, acc = eds + r * ds.abs(), f(lk) + f(lq)
+    gq, gk, gv = ds @ K * scale, ds.t() @ Q * scale, p.t() @ dO
+    res = {"out": (o, eo + u * o.abs()),
+           "dq": (gq, (edsr @ K.abs() + acc * (ds.abs() @ K.abs())) * scale + u * gq.abs()),
+           "dk": (gk, (edsr.t() @ Q.abs() + acc * (ds.abs().t() @ Q.abs())) * scale + u * gk.abs()),
+           "dv": (gv, (ep + r * p).t() @ dO.abs() + acc * (p.t() @ dO.abs()) + u * gv.abs())}
+    db, eb = (torch.zeros(n_buckets, dtype=torch.float64, device="cuda") for _ in range(2))
+    db.index_add_(0, slot.reshape(-1), ds.reshape(-1))
+    eb.index_add_(0, slot.reshape(-1), (eds + f(lk) * ds.abs()).reshape(-1))
+    res["dbias"] = (db, eb)
+    return res
+
+
+def check_gradients(q, k, v, dout, bias, table, qs, ks, causal, what, **hints):
+    """Every head of packed sequences (as many key heads as query heads) against one_head."""
+    from scenario_wise_rec import _hip as Hip
+    from scenario_wise_rec import ops
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, bias)]
+    out = ops.seq_attention(*leaves[:3], prefix(*qs), prefix(*ks), causal=causal, bias=leaves[3], buckets=table, **hints)
+    got = dict(zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(),) + torch.autograd.grad(out, leaves, dout)))
+    R = table.numel() - 1 if causal else table.numel() // 2
+    for h in range(q.shape[1]):
+        dbias, aq, ak = 0, 0, 0
+        for lq, lk in zip(qs, ks):
+            sq, sk = slice(aq, aq + lq), slice(ak, ak + lk)
+            dist = (torch.arange(lq, device="cuda") + lk - lq)[:, None] - torch.arange(lk, device="cuda")[None]
+            slot = table[dist.clamp(0, R) if causal else dist.clamp(-R, R) + R].long()
+            want = one_head(q[sq, h], k[sk, h], v[sk, h], dout[sq, h], bias[h][slot], slot, bias.shape[1], causal, q.shape[2] ** -0.5)
+            for n in ("out", "dq", "dk", "dv"):
+                ref.check(got[n][sk if n in ("dk", "dv") else sq, h], want[n], f"{what} head {h} {n}")
+            dbias = [a + b for a, b in zip(dbias, want["dbias"])] if dbias else list(want["dbias"])
+            aq, ak = aq + lq, ak + lk
+        ref.check(got["dbias"][h], dbias, f"{what} head {h} dbias")
+    Hip.check_errors()
+
+
+def both_sides(n, causal):
+    return one_each(n) if causal else torch.cat([one_each(n).flip(0), one_each(n)[1:]])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("value", [LOWEST, -1e9, 1e9, -1e6, -3000.0, 100.0])
+def test_gradients_of_rows_under_one_large_bias(value, D, causal, dtype):
+    """Head 0: every bucket holds the value (products of zero where it does not absorb them); head 1: ordinary biases."""
+    g, lens, H, n = gen(3), [150, 40], 2, 21
+    q, k, v, dout = (randn(g, 190, H, D, dtype=dtype) for _ in range(4))
+    if abs(value) < 1e9:
+        q[:, 0] = 0
+    bias = randn(g, H, n)
+    bias[0] = value
+    check_gradients(q, k, v, dout, bias, both_sides(n, causal), lens, lens, causal, str(value), max_q=150)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [LOWEST, -1e9])
+def test_gradients_where_some_rows_see_only_masked_buckets(value, dtype):
+    """Near distances under a large bias: the first rows of a causal sequence see nothing else and count alike, the rows behind them see
+    ordinary keys, and for them those keys are hidden.  Far distances the same way: there no row is left with them alone."""
+    g, L, H, D, n = gen(4), 140, 2, 32, 31
+    for near in (True, False):
+        q, k, v, dout = (randn(g, L, H, D, dtype=dtype) for _ in range(4))
+        bias = randn(g, H, n)
+        bias[:, :11 if near else 0] = value
+        if not near:
+            bias[:, 25:] = value
+        check_gradients(q, k, v, dout, bias, one_each(n), [L], [L], True, f"near {near}", max_q=L)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [LOWEST, -1e9, 1e9])
+def test_gradients_through_joined_key_ranges(value, dtype):
+    """A few queries over many keys, whose ranges are joined: the row's two parts come from the join."""
+    from scenario_wise_rec import _hip as Hip
+    g, qs, ks, H, D, n = gen(5), [3, 1], [2000, 700], 2, 64, 21
+    q, dout = randn(g, 4, H, D, dtype=dtype), randn(g, 4, H, D, dtype=dtype)
+    k, v = randn(g, 2700, H, D, dtype=dtype), randn(g, 2700, H, D, dtype=dtype)
+    bias = randn(g, H, n)
+    bias[0] = value
+    for causal in (True, False):
+        check_gradients(q, k, v, dout, bias, both_sides(n, causal), qs, ks, causal, "joined", max_q=3, max_k=2000)
+    a = Hip.SeqAttentionArgs()
+    a.Tq, a.Tk, a.B, a.Hq, a.Hk, a.D, a.dtype, a.causal, a.max_q, a.max_k = 4, 2700, 2, H, H, D, Hip.dtype_code(q), 1, 3, 2000
+    for name in ("q", "k", "v", "out", "cu_q", "cu_k"):
+        setattr(a, name, 4096)
+    assert Hip.lib.swr_seq_attention_fwd_workspace_bytes(Hip.C.byref(a)) > 0         # (ranges to join)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_of_large_scores(causal, dtype):
+    """Scores of 800, 804 and 808 without a bias: exact products, their weights are known.  800 log2 e = 1154: a rounding of 2^-14 in x and
+    in the row's exponent each, for a key and for the row's sum."""
+    g, L, H, D = gen(6), 90, 1, 16
+    q, k = torch.zeros(L, H, D, dtype=dtype, device="cuda"), torch.zeros(L, H, D, dtype=dtype, device="cuda")
+    q[..., 0] = 32.0
+    k[..., 0] = torch.randint(0, 3, (L, H), generator=g, device="cuda").to(dtype) / 2 + 100
+    v, dout = randn(g, L, H, D, dtype=dtype), randn(g, L, H, D, dtype=dtype)
+    from scenario_wise_rec import ops
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = ops.seq_attention(*leaves, prefix(L), max_q=L, causal=causal)
+    dv = torch.autograd.grad(out, leaves, dout)[2].double()[:, 0]
+    s = (q[:, 0].double() @ k[:, 0].double().t()) * 0.25
+    hidden = torch.arange(L, device="cuda")[:, None] < torch.arange(L, device="cuda")
+    p = torch.softmax(s.masked_fill(hidden & causal, float("-inf")), 1)
+    ep = (4 * 2.0 ** -14 + 2.0 ** -20) * p
+    r, u = (2.0 ** -8, 2.0 ** -8) if dtype == BF16 else (ref.f(16), 2.0 ** -24)
+    want, dO = p.t() @ dout[:, 0].double(), dout[:, 0].double().abs()
+    ref.check(dv, (want, (ep + r * p).t() @ dO + 2 * ref.f(L) * (p.t() @ dO) + u * want.abs()), "dv")
