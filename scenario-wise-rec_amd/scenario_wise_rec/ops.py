@@ -8,7 +8,7 @@ be strided (`ld = stride(0)`), so column slices of a wider buffer are passed wit
 import ctypes as C
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _hip as H
@@ -2715,6 +2715,12 @@ def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _no_tangents(what, *tensors):
+    """Reverse mode only: a dual tensor of forward-mode differentiation does not require grad, so it is looked for by itself."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivative is built (a tensor with a tangent was given)")
+
+
 def _unit_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -2844,6 +2850,7 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
     by key_mask may hold anything.  Differentiable in q, k, v and bias, deterministic.  Bad prefix sums, lengths and bucket ids are
     clamped and raise IndexError at the next `_hip.check_errors()`."""
     H.require_device(q, k, v, cu_q, bias)
+    _no_tangents("seq_attention", q, k, v, bias)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"seq_attention: q [Tq, Hq, D], k and v [Tk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _SEQ_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -2977,6 +2984,7 @@ def norm_gate_residual(x, y=None, gate=None, w_post=None, w_pre=None, scale=1.0,
     strided; w_post, w_pre: fp32 [N]; rms(a) = (mean a^2 + eps)^-1/2.  Returns z, or (z, u) with w_pre, or u alone with w_pre and
     without y (the norm before the first block).  Sums in fp32; u and the gradients start from the unrounded z."""
     H.require_device(x, y, gate, w_post, w_pre)
+    _no_tangents("norm_gate_residual", x, y, gate, w_post, w_pre)
     if x.dim() != 2 or x.shape[1] < 1 or x.shape[1] > H.NORM_GATE_MAX_WIDTH:
         raise ValueError(f"norm_gate_residual: x must be [M, N <= {H.NORM_GATE_MAX_WIDTH}], got {tuple(x.shape)}")
     if x.dtype not in _SEQ_TYPES:
