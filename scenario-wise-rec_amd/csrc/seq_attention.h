@@ -13,6 +13,7 @@
 // reader (16 consecutive rows, one piece each) and the transposing one (4 consecutive rows x 64 bytes per half wave).
 #pragma once
 #include "common.h"
+#include "seq_geometry.h"
 #include "split3.h"
 #include "vec8.h"
 
@@ -42,6 +43,7 @@ struct SaK {
     // launch geometry
     int tiles, per_unit, units, together;  // column tiles per sequence, workgroups per (sequence, key head), B * Hk, sa_unit
     int rest;                              // units behind the last: they write the rows of no sequence
+    unsigned blocks;                       // SaGrid's
     int pack;                              // query heads side by side in the columns (1 or G)
     int splits;                            // workgroups per key range
     float* part;                           // forward, splits > 1: [splits][Hq][Tq] (max, sum), then [splits][Hq][Tq][D]

@@ -16,7 +16,7 @@
 int sa_check(const swr_seq_attention_args* p, bool backward);
 SaK sa_args(const swr_seq_attention_args* p);
 int sa_waves(int64_t columns, const SaK& a, bool fp32);
-unsigned sa_grid(SaK& a);
+void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together);
 
 // waves per SIMD the registers are bounded for (512 / waves each)
 #define SA_WAVES_DQ(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : 2)
@@ -503,11 +503,9 @@ static SaBwdPlan sa_bwd_plan(const swr_seq_attention_args* p) {
     pl.q = pl.kv = sa_args(p);
     pl.nw_q = sa_waves(p->max_q, pl.q, p->dtype == SWR_F32);
     pl.nw_kv = sa_waves(p->max_k, pl.kv, p->dtype == SWR_F32);
-    pl.q.tiles = static_cast<int>(std::max<int64_t>(1, swr_ceil_div(p->max_q, pl.nw_q * 32)));
-    pl.kv.tiles = static_cast<int>(std::max<int64_t>(1, swr_ceil_div(p->max_k, pl.nw_kv * 32)));
-    pl.q.per_unit = pl.q.tiles * pl.q.G;
-    pl.kv.per_unit = pl.kv.tiles;
-    pl.fits = sa_grid(pl.q) && sa_grid(pl.kv);
+    sa_set_grid(pl.q, std::max<int64_t>(1, swr_ceil_div(p->max_q, pl.nw_q * 32)), pl.q.G, 0);
+    sa_set_grid(pl.kv, std::max<int64_t>(1, swr_ceil_div(p->max_k, pl.nw_kv * 32)), 1, 0);
+    pl.fits = pl.q.blocks && pl.kv.blocks;
     const int64_t slots = static_cast<int64_t>(p->B) * pl.q.tiles;
     pl.q.bias_slots = static_cast<int>(slots);
     pl.delta = static_cast<size_t>(p->Hq) * p->Tq * sizeof(float);
@@ -524,7 +522,7 @@ static int sa_dq_launch(SaK& a, hipStream_t st) {
     const int lds = SaDq<NP, DP, NW, FAST>::lds(a);
     SWR_REQUIRE(lds <= 160 * 1024, SWR_ERR_UNSUPPORTED);
     if (lds > 64 * 1024 && !swr_raise_lds(reinterpret_cast<const void*>(seq_attention_dq_kernel<NP, DP, NW, FAST>), 160 * 1024)) return SWR_ERR_LAUNCH;
-    hipLaunchKernelGGL((seq_attention_dq_kernel<NP, DP, NW, FAST>), dim3(sa_grid(a)), dim3(NW * 64), lds, st, a);
+    hipLaunchKernelGGL((seq_attention_dq_kernel<NP, DP, NW, FAST>), dim3(a.blocks), dim3(NW * 64), lds, st, a);
     return SWR_OK;
 }
 template <int NP, int DP, int NW, bool FAST>
@@ -532,7 +530,7 @@ static int sa_dkv_launch(SaK& a, hipStream_t st) {
     const int lds = SaDkv<NP, DP, NW, FAST>::lds(a);
     SWR_REQUIRE(lds <= 160 * 1024, SWR_ERR_UNSUPPORTED);
     if (lds > 64 * 1024 && !swr_raise_lds(reinterpret_cast<const void*>(seq_attention_dkv_kernel<NP, DP, NW, FAST>), 160 * 1024)) return SWR_ERR_LAUNCH;
-    hipLaunchKernelGGL((seq_attention_dkv_kernel<NP, DP, NW, FAST>), dim3(sa_grid(a)), dim3(NW * 64), lds, st, a);
+    hipLaunchKernelGGL((seq_attention_dkv_kernel<NP, DP, NW, FAST>), dim3(a.blocks), dim3(NW * 64), lds, st, a);
     return SWR_OK;
 }
 template <int NP, int DP>

@@ -359,17 +359,9 @@ int sa_waves(int64_t columns, const SaK& a, bool fp32) {
     return columns <= 32 ? 1 : (columns <= 64 ? 2 : 4);
 }
 
-// workgroups of a launch, or 0 when they do not fit a grid.  The rows of no sequence get units for at least 256 workgroups of their own.
-unsigned sa_grid(SaK& a) {
-    a.rest = (256 + a.per_unit - 1) / a.per_unit;
-    const int64_t each = (static_cast<int64_t>(a.units) + a.rest + 7) / 8;          // units per XCD
-    if (a.together <= 0 || a.together > each) a.together = static_cast<int>(each);
-    const int64_t slots = (each + a.together - 1) / a.together * a.together;
-    const int64_t max_per_unit = ((1ll << 30) / 8) / slots;
-    const int64_t rest = static_cast<int64_t>(a.per_unit / a.tiles);
-    if (rest > max_per_unit) return 0;
-    if (a.per_unit > max_per_unit) { a.tiles = static_cast<int>(max_per_unit / rest); a.per_unit = static_cast<int>(a.tiles * rest); }
-    return static_cast<unsigned>(slots * 8 * a.per_unit);
+void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together) {
+    const SaGrid g = sa_grid(a.units, tiles, inner, together);
+    a.tiles = g.tiles; a.per_unit = g.per_unit; a.rest = g.rest; a.together = g.together; a.blocks = g.blocks;
 }
 
 // Geometry of the forward.  pack: below 128 queries a workgroup of one head would leave columns empty while every head of the group
@@ -380,14 +372,12 @@ static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     const int64_t cols = static_cast<int64_t>(p->max_q) * a.pack;
     nw = sa_waves(cols, a, p->dtype == SWR_F32);
     const int64_t tiles = std::max<int64_t>(1, (cols + nw * 32 - 1) / (nw * 32));
-    a.tiles = static_cast<int>(std::min<int64_t>(tiles, 1 << 20));
-    const int64_t wgs = static_cast<int64_t>(a.units) * a.tiles * (a.G / a.pack);
+    const int64_t wgs = static_cast<int64_t>(a.units) * tiles * (a.G / a.pack);
     const int64_t key_tiles = (p->max_k + 63) / 64;
     a.splits = 1;
     const int64_t want = nw == 1 ? 4096 : 512;
     if (wgs > 0 && wgs < want) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
-    a.per_unit = a.tiles * (a.G / a.pack) * a.splits;
-    a.together = 1;
+    sa_set_grid(a, tiles, static_cast<int64_t>(a.G / a.pack) * a.splits, 1);
 }
 
 extern "C" size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_args* p) {
@@ -404,9 +394,7 @@ static int sa_fwd_launch(SaK& a, hipStream_t st) {
     const int lds = SaFwd<NP, DP, NW, FAST>::lds(a);
     const void* fn = reinterpret_cast<const void*>(seq_attention_fwd_kernel<NP, DP, NW, FAST, TRAIN>);
     if (lds > 64 * 1024 && !swr_raise_lds(fn, 160 * 1024)) return SWR_ERR_LAUNCH;
-    const unsigned grid = sa_grid(a);
-    SWR_REQUIRE(grid, SWR_ERR_UNSUPPORTED);
-    hipLaunchKernelGGL((seq_attention_fwd_kernel<NP, DP, NW, FAST, TRAIN>), dim3(grid), dim3(NW * 64), lds, st, a);
+    hipLaunchKernelGGL((seq_attention_fwd_kernel<NP, DP, NW, FAST, TRAIN>), dim3(a.blocks), dim3(NW * 64), lds, st, a);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.Hq) * a.Tq;
         hipLaunchKernelGGL((seq_attention_join_kernel<NP, DP>), dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, a);
@@ -432,6 +420,7 @@ extern "C" int swr_seq_attention_fwd(const swr_seq_attention_args* p, void* work
     SaK a = sa_args(p);
     int nw;
     sa_plan(p, a, nw);
+    SWR_REQUIRE(a.blocks, SWR_ERR_UNSUPPORTED);
     const size_t need = swr_seq_attention_fwd_workspace_bytes(p);
     if (need) {
         SWR_REQUIRE(workspace && workspace_bytes >= need, SWR_ERR_WORKSPACE);

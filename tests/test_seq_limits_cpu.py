@@ -20,3 +20,70 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
                    {"x": x, "w_pre": dual(w)}):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 ops.norm_gate_residual(**kw)
+
+
+GEOMETRY = r"""
+#include <cstdio>
+#include <vector>
+#include "seq_geometry.h"
+// sa_unit of the kernels
+static int unit_of(int id, const SaGrid& g, int& within) {
+    const int slot = id >> 3, round = slot / (g.per_unit * g.together), r = slot % (g.per_unit * g.together);
+    within = r / g.together;
+    return (round * g.together + r % g.together) * 8 + (id & 7);
+}
+int main() {
+    int bad = 0;
+    // every piece of work has one workgroup, so have the rows of no sequence
+    for (int64_t units : {0, 1, 7, 8, 300}) for (int64_t tiles : {1, 3, 40}) for (int64_t inner : {1, 5}) for (int64_t together : {0, 1, 3}) {
+        const SaGrid g = sa_grid(units, tiles, inner, together);
+        std::vector<int> hit((units + g.rest) * g.per_unit, 0);
+        for (unsigned id = 0; id < g.blocks; ++id) {
+            int within;
+            const int u = unit_of(id, g, within);
+            if (u < units + g.rest) ++hit[u * g.per_unit + within];
+        }
+        for (int h : hit) bad += h != 1;
+        bad += g.tiles != tiles || g.per_unit != tiles * inner || g.rest * g.per_unit < 256;
+    }
+    printf("small %d\n", bad);
+    // at the cap: tiles cut down, consistent in themselves, and the same when asked with what came out
+    const int64_t big[][3] = {{8000007, 500, 1}, {131072, 32, 4}, {524288, 16, 4}, {1 << 27, 1, 1}, {1 << 20, 1 << 26, 93}, {1, 1 << 26, 4096}, {(1 << 30) - 1, 1, 1}};
+    for (auto& c : big) for (int64_t together : {0, 1}) {
+        const SaGrid g = sa_grid(c[0], c[1], c[2], together);
+        if (!g.blocks) { printf("none\n"); continue; }
+        const SaGrid again = sa_grid(c[0], g.tiles, c[2], together);
+        printf("%d %d %d %u\n", g.tiles, g.per_unit == g.tiles * (int)c[2] && g.tiles >= 1, again.tiles == g.tiles && again.blocks >= g.blocks / 2, g.blocks);
+    }
+}
+"""
+
+
+def geometry(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "g.cpp").write_text(GEOMETRY)
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(root, "scenario-wise-rec_amd", "csrc"), str(tmp_path / "g.cpp"), "-o", str(tmp_path / "g")], check=True)
+    return subprocess.run([str(tmp_path / "g")], check=True, capture_output=True, text=True).stdout.split("\n")
+
+
+def test_launch_geometry_is_whole_and_computed_once(tmp_path):
+    """Every piece of work belongs to one workgroup; a launch cut down at the grid's cap is consistent with the tiles that partial sums
+    are laid out by, also when it is asked for again with them."""
+    lines = geometry(tmp_path)
+    assert lines[0] == "small 0"
+    cut = [line.split() for line in lines[1:] if line and line != "none"]
+    assert cut and all(c[1:3] == ["1", "1"] for c in cut), lines
+
+
+def test_backward_workspace_follows_the_launched_tiles():
+    """Partial sums of the bias gradient: one per bucket, sequence and launched tile, for a launch at the cap of the grid, too."""
+    from test_seq_ops_cpu import attention_args
+    import ctypes as C
+    from scenario_wise_rec import _hip as H
+    a = attention_args(B=8000007, Hq=1, Hk=1, Tq=64000, Tk=64000, max_q=64000, max_k=64, n_dist=9, n_buckets=4, bias=4096, buckets=4096,
+                       lse=4096, dout=4096, dq=4096, dk=4096, dv=4096, dbias=4096)
+    nbytes = H.lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
+    tiles, left = divmod(nbytes - 256 - 64000 * 4, 8000007 * 4 * 4)
+    assert left == 0 and 1 <= tiles <= 500
