@@ -16,7 +16,7 @@
 int sa_check(const swr_seq_attention_args* p, bool backward);
 SaK sa_args(const swr_seq_attention_args* p);
 int sa_waves(int64_t columns, const SaK& a, bool fp32);
-void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together);
+void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together, int waves);
 
 // waves per SIMD the registers are bounded for (512 / waves each)
 #define SA_WAVES_DQ(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : 2)
@@ -503,9 +503,9 @@ static SaBwdPlan sa_bwd_plan(const swr_seq_attention_args* p) {
     pl.q = pl.kv = sa_args(p);
     pl.nw_q = sa_waves(p->max_q, pl.q, p->dtype == SWR_F32);
     pl.nw_kv = sa_waves(p->max_k, pl.kv, p->dtype == SWR_F32);
-    sa_set_grid(pl.q, std::max<int64_t>(1, swr_ceil_div(p->max_q, pl.nw_q * 32)), pl.q.G, 0);
-    sa_set_grid(pl.kv, std::max<int64_t>(1, swr_ceil_div(p->max_k, pl.nw_kv * 32)), 1, 0);
-    pl.fits = pl.q.blocks && pl.kv.blocks;
+    sa_set_grid(pl.q, std::max<int64_t>(1, swr_ceil_div(p->max_q, pl.nw_q * 32)), pl.q.G, 0, pl.nw_q);
+    sa_set_grid(pl.kv, std::max<int64_t>(1, swr_ceil_div(p->max_k, pl.nw_kv * 32)), 1, 0, pl.nw_kv);
+    pl.fits = pl.q.blocks && pl.kv.blocks && static_cast<int64_t>(p->Hq) * p->n_buckets <= sa_most_blocks(256);
     const int64_t slots = static_cast<int64_t>(p->B) * pl.q.tiles;
     pl.q.bias_slots = static_cast<int>(slots);
     pl.delta = static_cast<size_t>(p->Hq) * p->Tq * sizeof(float);

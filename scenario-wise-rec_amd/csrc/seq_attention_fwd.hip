@@ -359,8 +359,8 @@ int sa_waves(int64_t columns, const SaK& a, bool fp32) {
     return columns <= 32 ? 1 : (columns <= 64 ? 2 : 4);
 }
 
-void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together) {
-    const SaGrid g = sa_grid(a.units, tiles, inner, together);
+void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together, int waves) {
+    const SaGrid g = sa_grid(a.units, tiles, inner, together, waves * 64);
     a.tiles = g.tiles; a.per_unit = g.per_unit; a.rest = g.rest; a.together = g.together; a.blocks = g.blocks;
 }
 
@@ -375,9 +375,9 @@ static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     const int64_t wgs = static_cast<int64_t>(a.units) * tiles * (a.G / a.pack);
     const int64_t key_tiles = (p->max_k + 63) / 64;
     a.splits = 1;
-    const int64_t want = nw == 1 ? 4096 : 512;
-    if (wgs > 0 && wgs < want) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
-    sa_set_grid(a, tiles, static_cast<int64_t>(a.G / a.pack) * a.splits, 1);
+    const int64_t want = nw == 1 ? 4096 : 512, rows = static_cast<int64_t>(a.Hq) * a.Tq;             // (rows: the join's grid)
+    if (wgs > 0 && wgs < want && (rows + 7) / 8 <= sa_most_blocks(256)) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
+    sa_set_grid(a, tiles, static_cast<int64_t>(a.G / a.pack) * a.splits, 1, nw);
 }
 
 extern "C" size_t swr_seq_attention_fwd_workspace_bytes(const swr_seq_attention_args* p) {
@@ -425,7 +425,6 @@ extern "C" int swr_seq_attention_fwd(const swr_seq_attention_args* p, void* work
     if (need) {
         SWR_REQUIRE(workspace && workspace_bytes >= need, SWR_ERR_WORKSPACE);
         SWR_REQUIRE(swr_aligned16(workspace), SWR_ERR_ALIGN);
-        SWR_REQUIRE(static_cast<int64_t>(a.Hq) * a.Tq / 8 < (1ll << 31) - 1, SWR_ERR_UNSUPPORTED);
         a.part = static_cast<float*>(workspace);
     }
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -10,16 +10,18 @@ struct SaGrid {
     int tiles, per_unit, rest, together;
     unsigned blocks;
 };
-// tiles: column tiles of the longest sequence; inner: workgroups of a tile (heads x key ranges); together <= 0: all units in one round
-static inline SaGrid sa_grid(int64_t units, int64_t tiles, int64_t inner, int64_t together) {
+// workgroups of `threads` that a launch takes: a grid has fewer than 2^32 threads
+static inline int64_t sa_most_blocks(int threads) { return ((1ll << 32) - 1) / threads; }
+// tiles: column tiles of the longest sequence; inner: workgroups of a tile (heads x key ranges); together <= 0: all units in one round;
+// threads: of a workgroup
+static inline SaGrid sa_grid(int64_t units, int64_t tiles, int64_t inner, int64_t together, int threads) {
     SaGrid g{};
-    const int64_t most = 1ll << 30;
     int64_t per_unit = tiles * inner;
     const int64_t rest = (256 + per_unit - 1) / per_unit;
     const int64_t each = (units + rest + 7) / 8;                   // units of an XCD
     if (together <= 0 || together > each) together = each;
     const int64_t slots = (each + together - 1) / together * together;
-    const int64_t room = most / 8 / slots;                         // workgroups a unit may have
+    const int64_t room = sa_most_blocks(threads) / 8 / slots;                         // workgroups a unit may have
     if (inner > room) return g;
     if (per_unit > room) { tiles = room / inner; per_unit = tiles * inner; }
     g.tiles = static_cast<int>(tiles);

@@ -36,7 +36,7 @@ int main() {
     int bad = 0;
     // every piece of work has one workgroup, so have the rows of no sequence
     for (int64_t units : {0, 1, 7, 8, 300}) for (int64_t tiles : {1, 3, 40}) for (int64_t inner : {1, 5}) for (int64_t together : {0, 1, 3}) {
-        const SaGrid g = sa_grid(units, tiles, inner, together);
+        const SaGrid g = sa_grid(units, tiles, inner, together, 64);
         std::vector<int> hit((units + g.rest) * g.per_unit, 0);
         for (unsigned id = 0; id < g.blocks; ++id) {
             int within;
@@ -49,11 +49,12 @@ int main() {
     printf("small %d\n", bad);
     // at the cap: tiles cut down, consistent in themselves, and the same when asked with what came out
     const int64_t big[][3] = {{8000007, 500, 1}, {131072, 32, 4}, {524288, 16, 4}, {1 << 27, 1, 1}, {1 << 20, 1 << 26, 93}, {1, 1 << 26, 4096}, {(1 << 30) - 1, 1, 1}};
-    for (auto& c : big) for (int64_t together : {0, 1}) {
-        const SaGrid g = sa_grid(c[0], c[1], c[2], together);
+    for (auto& c : big) for (int64_t together : {0, 1}) for (int threads : {64, 128, 256}) {
+        const SaGrid g = sa_grid(c[0], c[1], c[2], together, threads);
         if (!g.blocks) { printf("none\n"); continue; }
-        const SaGrid again = sa_grid(c[0], g.tiles, c[2], together);
-        printf("%d %d %d %u\n", g.tiles, g.per_unit == g.tiles * (int)c[2] && g.tiles >= 1, again.tiles == g.tiles && again.blocks >= g.blocks / 2, g.blocks);
+        const SaGrid again = sa_grid(c[0], g.tiles, c[2], together, threads);
+        printf("%d %d %d %d %u\n", g.tiles, g.per_unit == g.tiles * (int)c[2] && g.tiles >= 1, again.tiles == g.tiles && again.blocks >= g.blocks / 2,
+               (long long)g.blocks * threads < (1ll << 32), g.blocks);
     }
 }
 """
@@ -75,6 +76,7 @@ def test_launch_geometry_is_whole_and_computed_once(tmp_path):
     assert lines[0] == "small 0"
     cut = [line.split() for line in lines[1:] if line and line != "none"]
     assert cut and all(c[1:3] == ["1", "1"] for c in cut), lines
+    assert all(c[3] == "1" for c in cut), lines                      # (fewer than 2^32 threads)
 
 
 def test_backward_workspace_follows_the_launched_tiles():
@@ -87,3 +89,23 @@ def test_backward_workspace_follows_the_launched_tiles():
     nbytes = H.lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
     tiles, left = divmod(nbytes - 256 - 64000 * 4, 8000007 * 4 * 4)
     assert left == 0 and 1 <= tiles <= 500
+
+
+def test_launches_of_many_sequences_stay_below_the_grid_limit():
+    """Many sequences with one long one among them: fewer tiles are launched (and walked in more rounds), not more threads than a grid takes.
+    More sequences than workgroups fit are refused."""
+    from test_seq_ops_cpu import attention_args
+    import ctypes as C
+    from scenario_wise_rec import _hip as H
+    back = dict(lse=4096, dout=4096, dq=4096, dk=4096, dv=4096)
+    tab = dict(n_dist=9, n_buckets=4, bias=4096, buckets=4096, dbias=4096)
+    for B, Hk, G, longest in ((16384, 8, 4, 4096), (65536, 4, 4, 2048)):
+        a = attention_args(B=B, Hq=Hk * G, Hk=Hk, Tq=1 << 20, Tk=1 << 20, max_q=longest, max_k=longest, D=64, **back, **tab)
+        nbytes = H.lib.swr_seq_attention_bwd_workspace_bytes(C.byref(a))
+        tiles, left = divmod(nbytes - 256 - (1 << 22) * Hk * G, B * 4 * Hk * G * 4)
+        assert left == 0 and 1 <= tiles and B * Hk * G * tiles * 256 < 1 << 32
+    a = attention_args(B=1 << 26, Hq=1, Hk=1, **back)
+    assert H.lib.swr_seq_attention_fwd(C.byref(a), None, 0, None) == -5 and H.lib.swr_seq_attention_bwd(C.byref(a), None, 0, None) == -5
+    # (two million rows of 93 heads: the launch that joins key ranges would not fit, so none are made)
+    a = attention_args(Tq=1 << 21, B=1, Hq=93, Hk=1, max_q=1, Tk=20000, max_k=20000)
+    assert H.lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a)) == 0

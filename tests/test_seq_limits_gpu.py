@@ -24,3 +24,34 @@ def test_calls_without_tangents_inside_a_forward_mode_level():
         dual = forward_ad.make_dual(q, torch.ones_like(q))
         with pytest.raises(NotImplementedError):
             ops.seq_attention(dual, q, q, cu)
+
+
+def test_many_sequences_and_one_long():
+    """More workgroups than a grid takes if each sequence got the long one's: 65 536 of up to two rows, one of 2 048."""
+    from scenario_wise_rec import _hip as H
+    from scenario_wise_rec import ops
+    B, Hq, Hk, D = 65536, 16, 4, 8
+    lens = torch.ones(B, dtype=torch.int64)
+    lens[::7] = 2
+    lens[::11] = 0
+    lens[40001] = 2048
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
+    T = int(cu[-1])
+    q, k, v, dout = randn(3, T, Hq, D), randn(4, T, Hk, D), randn(5, T, Hk, D), randn(6, T, Hq, D)
+    bias, table = randn(7, Hq, 4), torch.arange(4, dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v, bias)]
+    out = ops.seq_attention(*leaves[:3], cu.to(torch.int32).cuda(), max_q=2048, bias=bias, buckets=table)
+    got = dict(zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(),) + torch.autograd.grad(out, leaves, dout)))
+    H.check_errors()
+    leaves = [t.detach() for t in leaves]
+    a, n = int(cu[40001]), 2048
+    some = [(a, n)] + [(int(cu[b]), int(lens[b])) for b in (0, 1, 2, 3, 7, 11, 40000, 40002, B - 2, B - 1)]
+    qs, q0 = [s[1] for s in some], [s[0] for s in some]
+    want = ref.attention(*leaves[:3], dout, qs, qs, q0, q0, True, None, leaves[3], table)
+    for name in ("out", "dq", "dk", "dv"):
+        rows = torch.cat([torch.arange(s, s + n) for s, n in some]).cuda()
+        ref.check(got[name][rows], tuple(t[rows] for t in want[name]), name)
+    # the short ones by hand: one row attends to itself, out = v
+    one = cu[:-1][lens == 1].cuda()
+    assert torch.equal(out.detach()[one], v.detach()[one].repeat_interleave(Hq // Hk, 1))
+    assert torch.isfinite(got["dbias"]).all()
