@@ -372,10 +372,12 @@ static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     const int64_t cols = static_cast<int64_t>(p->max_q) * a.pack;
     nw = sa_waves(cols, a, p->dtype == SWR_F32);
     const int64_t tiles = std::max<int64_t>(1, (cols + nw * 32 - 1) / (nw * 32));
-    const int64_t wgs = static_cast<int64_t>(a.units) * tiles * (a.G / a.pack);
+    // (as many as max_q says, or as the rows there are fill: with a max_q below the mean the ranges' workspace would follow the rows)
+    const int64_t rows = static_cast<int64_t>(a.Hq) * a.Tq;
+    const int64_t wgs = std::max(static_cast<int64_t>(a.units) * tiles * (a.G / a.pack), (rows + nw * 32 - 1) / (nw * 32));
     const int64_t key_tiles = (p->max_k + 63) / 64;
     a.splits = 1;
-    const int64_t want = nw == 1 ? 4096 : 512, rows = static_cast<int64_t>(a.Hq) * a.Tq;             // (rows: the join's grid)
+    const int64_t want = nw == 1 ? 4096 : 512;
     if (wgs > 0 && wgs < want && (rows + 7) / 8 <= sa_most_blocks(256)) a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, key_tiles / (wgs < 512 ? 2 : 8), 64})));
     sa_set_grid(a, tiles, static_cast<int64_t>(a.G / a.pack) * a.splits, 1, nw);
 }

@@ -109,3 +109,15 @@ def test_launches_of_many_sequences_stay_below_the_grid_limit():
     # (two million rows of 93 heads: the launch that joins key ranges would not fit, so none are made)
     a = attention_args(Tq=1 << 21, B=1, Hq=93, Hk=1, max_q=1, Tk=20000, max_k=20000)
     assert H.lib.swr_seq_attention_fwd_workspace_bytes(C.byref(a)) == 0
+
+
+def test_a_max_q_below_the_mean_does_not_blow_up_the_workspace():
+    """The hint is right for any value: one sequence of a million queries called with max_q = 1 asked for 64 key ranges of every row."""
+    from test_seq_ops_cpu import attention_args
+    import ctypes as C
+    from scenario_wise_rec import _hip as H
+    need = lambda **kw: H.lib.swr_seq_attention_fwd_workspace_bytes(C.byref(attention_args(**kw)))
+    for dtype in (H.F32, H.BF16):
+        for rows in (1, 100, 5000, 1 << 17, 1 << 20):
+            assert need(dtype=dtype, B=1, Tq=rows, max_q=1, Tk=1 << 20, max_k=1 << 20) <= 1 << 27, rows
+    assert need(B=1, Tq=1, max_q=1, Tk=20000, max_k=20000) > 0                   # (an honest hint still splits the keys)
