@@ -861,8 +861,8 @@ int swr_seq_attention_bwd(const swr_seq_attention_args* a, void* workspace, size
  *   u = z rms(z) w_pre     (w_pre NULL: no u)           z enters unrounded
  * Rows of N <= SWR_NORM_GATE_MAX_WIDTH elements of `dtype` (SWR_F32 / SWR_BF16); x, y, gate, dz, du have leading dimensions, z, u, dx,
  * dy, dgate are contiguous; weights, their gradients and ry / rz ([M], kept for the backward; nullable in a forward without one) fp32.
- * Backward: dz and du nullable (a missing one counts as zeros), dx, dy, dgate overwritten, dw_post / dw_pre nullable, fixed-order
- * column sums (accumulate = 1 adds into them -- gradient arena; workspace needed when one of them is asked for). */
+ * Backward: ry with w_post, rz with w_pre; dz and du nullable (a missing one counts as zeros), dx, dy, dgate overwritten, dw_post /
+ * dw_pre nullable, fixed-order column sums (accumulate = 1 adds into them -- gradient arena; workspace needed when one is asked for). */
 #define SWR_NORM_GATE_MAX_WIDTH 8192
 typedef struct {
     int64_t M;

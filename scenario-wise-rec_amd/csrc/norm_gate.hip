@@ -299,7 +299,7 @@ static int ng_check(const swr_norm_gate_args* p, bool backward) {
         SWR_REQUIRE((!p->y || p->z) && (!p->w_pre || p->u), SWR_ERR_ARG);
     } else {
         SWR_REQUIRE(p->dx && (!p->y || p->dy) && (!p->gate || p->dgate) && (p->dz || p->du), SWR_ERR_ARG);
-        SWR_REQUIRE((!p->du || (p->w_pre && p->rz)) && (!p->w_post || p->ry), SWR_ERR_ARG);
+        SWR_REQUIRE((!p->du || p->w_pre) && (!p->w_pre || p->rz) && (!p->w_post || p->ry), SWR_ERR_ARG);
     }
     return SWR_OK;
 }

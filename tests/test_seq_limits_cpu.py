@@ -121,3 +121,15 @@ def test_a_max_q_below_the_mean_does_not_blow_up_the_workspace():
         for rows in (1, 100, 5000, 1 << 17, 1 << 20):
             assert need(dtype=dtype, B=1, Tq=rows, max_q=1, Tk=1 << 20, max_k=1 << 20) <= 1 << 27, rows
     assert need(B=1, Tq=1, max_q=1, Tk=20000, max_k=20000) > 0                   # (an honest hint still splits the keys)
+
+
+def test_norm_backward_refuses_a_missing_row_statistic():
+    """The kernel reads rz wherever w_pre is given, with or without du; a NULL there was a read through it."""
+    import ctypes as C
+    from scenario_wise_rec import _hip as H
+    a = H.NormGateArgs()
+    for name, value in dict(M=8, N=64, dtype=H.F32, x=4096, y=4096, w_pre=4096, dz=4096, dx=4096, dy=4096, dw_post=4096).items():
+        setattr(a, name, value)
+    assert H.lib.swr_norm_gate_bwd(C.byref(a), None, 0, None) == -1
+    a.rz = 4096                                            # (the next check is the workspace's)
+    assert H.lib.swr_norm_gate_bwd(C.byref(a), None, 0, None) == -6
