@@ -128,6 +128,8 @@ def _plan_part(plan, weights, wpos, layer, x, sparse, dense):
             if idx.dim() != 2:
                 raise ValueError(f"sequence feature {fea.name!r}: expected ids of shape (batch_size, seq_len), got {tuple(idx.shape)}")
             mode = {"sum": 0, "mean": 1, "concat": 2, "attention": 2}[fea.pooling]
+            if fea.pooling == "attention" and fea.padding_idx is None:
+                idx = idx.masked_fill(idx == -1, 0)            # (padding: looked up as any row, hidden from the block)
             plan.bags.append({"wpos": wpos[key], "idx": idx, "vocab": w.shape[0], "dim": w.shape[1], "col": col,
                               "L": idx.shape[1], "mode": mode, "pad": fea.padding_idx, "seed": getattr(fea, "hash_seed", 0)})
             col += w.shape[1] * (idx.shape[1] if mode == 2 else 1)

@@ -55,3 +55,36 @@ def test_many_sequences_and_one_long():
     one = cu[:-1][lens == 1].cuda()
     assert torch.equal(out.detach()[one], v.detach()[one].repeat_interleave(Hq // Hk, 1))
     assert torch.isfinite(got["dbias"]).all()
+
+
+@pytest.mark.parametrize("hash_seed", [0, 7])
+def test_attention_pooling_of_minus_one_padding(hash_seed):
+    """Without a padding_idx the padding is -1, as for the other poolings: not an id, not looked up, no gradient."""
+    from scenario_wise_rec import _hip as H
+    from scenario_wise_rec.basic.features import SequenceFeature
+    from scenario_wise_rec.basic.layers import EmbeddingLayer
+    H.check_errors()
+
+    def layer(pad):
+        torch.manual_seed(1)
+        f = [SequenceFeature("h", 40, 16, pooling="attention", padding_idx=pad, hash_seed=hash_seed, attention={"n_heads": 2, "max_distance": 16})]
+        m = EmbeddingLayer(f)
+        with torch.no_grad():
+            m.embed_dict["h"].weight.normal_(0, 0.5)
+        return f, m.to("cuda").train()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    ids = torch.randint(1, 40, (30, 7), generator=g, device="cuda")
+    hidden = torch.rand(30, 7, generator=g, device="cuda") < 0.4
+    hidden[3] = True
+    d = torch.randn(30, 16, generator=g, device="cuda")
+    res = []
+    for pad, value in ((0, 0), (None, -1)):                       # (id 0 is nobody's in this batch: the two mean the same)
+        f, m = layer(pad)
+        out = m({"h": ids.masked_fill(hidden, value)}, f, squeeze_dim=True)
+        out.backward(d)
+        H.check_errors()
+        res.append([out.detach()] + [p.grad for p in m.parameters()])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+    assert not res[1][0][3].any() and torch.isfinite(res[1][0]).all()
