@@ -88,3 +88,42 @@ def test_attention_pooling_of_minus_one_padding(hash_seed):
     for a, b in zip(*res):
         assert torch.equal(a, b)
     assert not res[1][0][3].any() and torch.isfinite(res[1][0]).all()
+
+
+@pytest.mark.parametrize("family", ["SharedBottom", "MMOE", "PLE", "Star", "HamurSmall", "HamurLarge", "M3oE"])
+def test_every_model_that_looks_up_through_the_embedding_layer(family):
+    """An attention-pooled history in each of them: a step runs and every parameter of the block gets a gradient."""
+    from scenario_wise_rec import _hip as H
+    from scenario_wise_rec.basic.features import SequenceFeature, SparseFeature
+    from scenario_wise_rec.models import multi_domain as md
+    from scenario_wise_rec.trainers import CTRTrainer
+    D, B = 3, 300
+    feats = [SparseFeature("s0", 17, 16), SequenceFeature("h", 60, 16, pooling="attention", padding_idx=0, attention={"n_heads": 2, "max_distance": 16}),
+             SparseFeature("s1", 900, 16), SequenceFeature("m", 30, 16, pooling="mean", padding_idx=0)]
+    deep = {"expert_params": {"dims": [16]}, "tower_params": {"dims": [8]}}
+    torch.manual_seed(3)
+    model = {"SharedBottom": lambda: md.SharedBottom(feats, domain_num=D, bottom_params={"dims": [32]}, tower_params={"dims": [8]}),
+             "MMOE": lambda: md.MMOE(feats, domain_num=D, n_expert=2, **deep),
+             "PLE": lambda: md.PLE(feats, domain_num=D, n_level=1, n_expert_specific=2, n_expert_shared=1, **deep),
+             "Star": lambda: md.Star(feats, D, [32, 16], [16]),
+             "HamurSmall": lambda: md.HamurSmall(feats, D, [32, 16], [16], 8),
+             "HamurLarge": lambda: md.HamurLarge(feats, D, [32, 16, 16, 16, 16, 16, 16], [16], 8),
+             "M3oE": lambda: md.M3oE(feats, domain_num=D, fcn_dims=[32, 16, 16, 8], expert_num=2, exp_d=1, exp_t=1, bal_d=1, bal_t=1, device="cuda")}[family]()
+    with torch.no_grad():
+        for n, w in model.named_parameters():
+            if "embed_dict" in n or "position" in n:
+                w.normal_(0, 0.3)
+    trainer = CTRTrainer(model, "attention", optimizer_params={"lr": 1e-3, "weight_decay": 1e-5}, device="cuda")
+    model.train()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    ids = lambda hi, *s: torch.randint(0, hi, s, generator=g, device="cuda")
+    x = {"s0": ids(17, B), "s1": ids(900, B), "h": ids(60, B, 9), "m": ids(30, B, 4), "domain_indicator": ids(D, B)}
+    y = (torch.rand(B, generator=g, device="cuda") < 0.3).float()
+    model.zero_grad()
+    trainer.criterion(model(x), y).backward()
+    for n, w in model.named_parameters():
+        if "seq_blocks" in n:
+            assert w.grad is not None and torch.isfinite(w.grad).all() and w.grad.any(), n
+    trainer.train_step(x, y)
+    H.check_errors()
