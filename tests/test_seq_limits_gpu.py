@@ -127,3 +127,41 @@ def test_every_model_that_looks_up_through_the_embedding_layer(family):
             assert w.grad is not None and torch.isfinite(w.grad).all() and w.grad.any(), n
     trainer.train_step(x, y)
     H.check_errors()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("D", [4, 16, 20, 33, 64, 128])
+def test_hidden_keys_and_rows_in_use_at_every_width(D, aligned, causal, dtype):
+    """A padded batch with hidden keys, unused rows behind q_len and NaN in all of them, walked in one and in several rounds, in every width's
+    kernels and for rows off every alignment."""
+    from scenario_wise_rec import _hip as H
+    from scenario_wise_rec import ops
+    B, L, Hq, Hk = 3, 150, 4, 2
+    used = [150, 97, 0]
+    lens, at = torch.tensor(used, dtype=torch.int32, device="cuda"), [0, 150, 300]
+    mask = torch.rand(B * L, generator=torch.Generator("cuda").manual_seed(8), device="cuda") < 0.6
+    mask[:40] = False                                  # (causal: the first rows see nothing)
+    unused = torch.cat([torch.arange(L, device="cuda") >= n for n in used])
+    def rows(seed, heads):
+        t = randn(seed, B * L, heads, D, dtype=dtype)
+        if not aligned:
+            wide = torch.empty(B * L * heads * (D + 1) + 1, dtype=dtype, device="cuda")[1:].view(B * L, heads, D + 1)[..., :D]
+            t = wide.copy_(t)
+        return t
+    q, k, v, dout = rows(1, Hq), rows(2, Hk), rows(3, Hk), rows(4, Hq)
+    for t in (q, dout):
+        t[unused] = float("nan")
+    for t in (k, v):
+        t[unused | ~mask] = float("nan")
+    bias, table = randn(5, Hq, 8), ops.seq_buckets(8, 30, causal)
+    want = ref.attention(q, k, v, dout, used, used, at, at, causal, None, bias, table, mask)
+    for hint in (150, 1):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, bias)]
+        out = ops.seq_attention(*leaves[:3], torch.tensor([0, 150, 300, 450], dtype=torch.int32, device="cuda"), max_q=hint, causal=causal,
+                                bias=leaves[3], buckets=table, key_mask=mask, q_len=lens)
+        got = dict(zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(),) + torch.autograd.grad(out, leaves, dout)))
+        for n, t in got.items():
+            ref.check(t, want[n], f"{n} hint {hint}")
+    H.check_errors()
