@@ -1,5 +1,5 @@
 // Stand-alone timing harness of dw_tr_kernel (csrc/dw_tr.hip) at config 2's shape with synthetic operands: no python, no torch.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Iinclude -Iscenario-wise-rec_amd/csrc [-DDT_STAMPS ...] tools/micro/dw_tr_harness.hip -o tools/micro/bin/dw_tr_harness
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -Iinclude -Iscenario-wise-rec_amd/csrc [-DDT_STAMPS ...] tools/micro/dw_tr_harness.hip -o tools/micro/bin/dw_tr_harness
 // Prints the mean kernel time over 50 launches (HIP events) and, with -DDT_STAMPS, the shader-clock stamps of workgroup 0 / wave 0
 // (prologue end, every stage end, kernel end).  Results are not checked here (tools/micro/dw_probe.py does that through the C ABI).
 #include "../../scenario-wise-rec_amd/csrc/dw_tr.hip"

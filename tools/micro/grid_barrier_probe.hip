@@ -1,7 +1,7 @@
 // Cost and correctness of a hand-rolled grid barrier on gfx950 (8 XCDs, one L2 each): NWG resident workgroups run NB rounds of
 //   write one partial per workgroup (+ DIRTY bytes of other stores, to load the L2 write-back a release has to do)
 //   -> barrier -> read ALL partials and compare with the value every workgroup must have written this round.
-// Prints us per round and the number of stale reads (must be 0).  Build: hipcc --offload-arch=gfx950 -O3 -o gbp grid_barrier_probe.hip
+// Prints us per round and the number of stale reads (must be 0).  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o gbp grid_barrier_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
