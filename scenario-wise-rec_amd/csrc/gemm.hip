@@ -778,7 +778,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void gemm_tn_kernel(const TnK kk) 
 #pragma unroll
             for (int tb = 0; tb < TN_TB; ++tb)
                 acc[ta][tb] = __builtin_amdgcn_mfma_f32_32x32x2f32(f.a[ta], f.b[tb], acc[ta][tb], 0, 0, 0);
-        // column sums as opaque scalar adds: left to the SLP vectoriser they become v_pk_add_f32 on register pairs
+        // column sums as opaque scalar adds: left to the SLP vectoriser they are gathered into register pairs
         // assembled with v_mov from freshly loaded ring slots, which forces a wait on nearly every load in flight
 #pragma unroll
         for (int t = 0; t < TA; ++t) asm volatile("v_add_f32 %0, %0, %1" : "+v"(cs[t]) : "v"(f.a[t]));

@@ -18,7 +18,9 @@ SaK sa_args(const swr_seq_attention_args* p);
 int sa_waves(int64_t columns, const SaK& a, bool fp32);
 void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together, int waves);
 
-// waves per SIMD the registers are bounded for (512 / waves each)
+// waves per SIMD the registers are bounded for (512 / waves each): as many as spill nothing -- one more spills in every kernel that has
+// not got its registers anyway, but in those of one or two waves at DP = 128, bf16, which take one (steps of 512 histories, 8 heads, one
+// against two: up to 60 rows 281 / 241 us, up to 30 rows 200 / 204)
 #define SA_WAVES_DQ(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : 2)
 #define SA_WAVES_DKV(NP, DP, NW, FAST) ((NP) * (DP) >= 192 || ((DP) == 128 && ((NW) < 4 || !(FAST))) ? 1 : ((NP) * (DP) == 32 ? 3 : 2))
 #define SA_PITCH 36                            // a wave's skewed 32 x 32 block: one row per distance (63, and one of zeros), 32 keys

@@ -14,7 +14,8 @@
 
 #include "seq_attention.h"
 
-// waves per SIMD the registers are bounded for (512 / waves each)
+// waves per SIMD the registers are bounded for (512 / waves each): as many as spill nothing.  (One wave a workgroup at DP = 64, fp32, and at
+// DP = 128, bf16, would bear one more; these are launches of few columns, whose workgroups do not fill the chip.)
 #define SA_WAVES(NP, DP, NW) ((NP) * (DP) >= 384 || ((NP) * (DP) == 192 && (NW) < 4) || ((NP) * (DP) == 128 && (NW) == 1) ? 1 : (((DP) == 32 && (NW) == 1) || (NP) * (DP) == 64 ? 3 : 2))
 
 template <int NP, int DP, int NW, bool FAST>
@@ -350,9 +351,12 @@ SaK sa_args(const swr_seq_attention_args* p) {
     return a;
 }
 
-// waves of 32 columns per workgroup: as many as the longest sequence fills, at most four.  fp32 rows above 64 columns always take
-// four: the registers that stage a tile (and double by half the waves) do not fit beside the operands'.  So do rows that are not
-// 16-byte aligned (one variant for all of them).
+// waves of 32 columns per workgroup: as many as the longest sequence fills, at most four.  fp32 rows of up to 32 columns take one wave for
+// up to 256 query columns: no wave of a workgroup waits for the others' tiles, and a short sequence leaves none idle.  Measured, one wave
+// against up to four: training steps of 1 024 histories up to 50, 4 heads of 16, 118 / 144 us, 512 up to 200 213 / 277, 512 up to 200,
+// 8 heads of 32, 398 / 520; where few sequences leave the chip empty it loses: 64 of 200 to 256 98 / 71, 16 of 100 to 256 72 / 61.
+// fp32 rows above 64 columns always take four: the registers that stage a tile (and double by half the waves) do not fit beside the
+// operands'.  So do rows that are not 16-byte aligned (one variant for all of them).
 int sa_waves(int64_t columns, const SaK& a, bool fp32) {
     if (!a.fast || (fp32 && a.D > 64)) return 4;
     if (fp32 && a.D <= 32 && a.pack == 1 && columns <= 256) return 1;
@@ -365,8 +369,11 @@ void sa_set_grid(SaK& a, int64_t tiles, int64_t inner, int64_t together, int wav
 }
 
 // Geometry of the forward.  pack: below 128 queries a workgroup of one head would leave columns empty while every head of the group
-// reads the same keys, so the group's heads share the columns.  splits: workgroups are added along the keys until the 256 CUs hold
-// two each, as long as a range keeps two tiles.
+// reads the same keys, so the group's heads share the columns.  splits: workgroups are added along the keys until there are 512 (two a
+// CU), 4 096 of one-wave workgroups (a SIMD holds more than one, and each has little in flight); a range keeps two tiles of 64 keys, eight
+// where there were 512 workgroups already.  Measured: 4 096 against 512 for one-wave workgroups, a token for each of 128 caches of 1 000,
+// fp32, 4 heads of 16, 39 / 62 us, but of 8 caches of 4 000 41 / 34, bf16, 32/8 heads of 128, 8 of 4 000 60 / 39, 128 of 4 000 373 / 352;
+// eight against two tiles from 512 on, the 128 of 1 000 39 / 46, bf16 32 of 4 000 132 / 128.
 static void sa_plan(const swr_seq_attention_args* p, SaK& a, int& nw) {
     a.pack = a.G > 1 && p->max_q < 128 && p->Tq * a.G < (1ll << 31) - 4096 ? a.G : 1;
     const int64_t cols = static_cast<int64_t>(p->max_q) * a.pack;

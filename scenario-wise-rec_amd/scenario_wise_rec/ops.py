@@ -2846,6 +2846,10 @@ def seq_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=True,
     max_q / max_k: the longest sequence if known on the host (chooses the launch and its tiling, right for any value; default: four
     times the mean).
 
+    Scores are held in fp32: a bias of large magnitude (-1e9, the lowest value) hides its keys from rows that see others, and in a row
+    where every visible key carries it they weigh alike.  bf16: the probabilities enter their product rounded to bf16, in two terms where
+    a gradient is recorded -- the same inputs round differently with and without one, by 2^-9 of the values.
+
     A row without a visible key, and rows of no sequence or beyond q_len, are zeros with zero gradients; keys beyond k_len or hidden
     by key_mask may hold anything.  Differentiable in q, k, v and bias, deterministic.  Bad prefix sums, lengths and bucket ids are
     clamped and raise IndexError at the next `_hip.check_errors()`."""
