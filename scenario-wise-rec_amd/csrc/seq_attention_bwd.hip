@@ -102,6 +102,12 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
         const int64_t row = sq.q0 + (exists ? tok : 0), at = static_cast<int64_t>(h) * n->Tq + row;
         bf16x8 Q[DP / 16][NP], dO[DP / 16][NP];
         sa_row_frags<NP, DP, FAST>(n->q, row * n->q_row + static_cast<int64_t>(h) * n->q_head, live, a.D, n->vq, lane, Q);
+        // fp32: odd rows enter the product do . v with their signs flipped and leave it flipped back.  The matrix pipe's sums are rounded
+        // down (3e-8 on average per row of 16 columns of N(0, 1) values): that drifts into the bias gradient, whose other terms cancel in
+        // every row, and with alternating signs it cancels between rows (1 024 histories up to 50: off by 1.2e-6 / 1.7e-7 of its norm,
+        // 512 up to 200 1.5e-6 / 2.4e-7, the same times).  On bf16 tensors the two terms of the forward's probabilities leave 1.5e-6 either
+        // way, and at 128 columns the flips cost 1 %.
+        const int odd = static_cast<int>(sq.q0 + wfirst) & 1;              // (of the row of lane 0: a column's row is odd where lane ^ odd is)
         float delta = 0.f;
         const int hi8 = sa_here(8 * hi);
 #pragma unroll
@@ -114,7 +120,13 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
             floats8(y, fy);
 #pragma unroll
             for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
-            sa_planes(x, dO[s]);
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) fx[j] = (lane ^ odd) & 1 ? -fx[j] : fx[j];
+                sa_split8(fx, dO[s]);
+            } else {
+                sa_planes(x, dO[s]);
+            }
         }
         delta += __shfl_xor(delta, 32);
         const float lse = live ? n->lse[at] : INFINITY;
@@ -176,16 +188,17 @@ __global__ __launch_bounds__(NW * 64, SA_WAVES_DQ(NP, DP, NW, FAST)) void seq_at
                 cols(0, 0);
                 const int near_d = wfirst + sq.shift - (k0 + 31), far_d = wlast + sq.shift - k0;
                 const SaSpan sp = sa_span(a, near_d, far_d);
+                const float sign = NP == 3 ? __uint_as_float(0x3f800000u | (static_cast<uint32_t>(sa_here(threadIdx.x) ^ odd) << 31)) : 1.f;
                 if (sp.apart && !parts) {
                     const float add = (a.row ? bt[sp.entry] : 0.f) - lse;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + add) * (dP[i] - delta);
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(S[i] * a.c + add) * (dP[i] * sign - delta);
                 } else {
                     const float* be = bt + (sp.apart ? sa_flat_entry(a, sp) : sa_entry(a, qpos - k0 - 4 * hi - 27));
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float p = __builtin_amdgcn_exp2f((S[i] * a.c + be[27 - 8 * (i >> 2) - (i & 3)]) - lse);
-                        S[i] = p * (dP[i] - delta);
+                        S[i] = p * (dP[i] * sign - delta);
                     }
                     if (parts) {
                         const SaArgs n = sa_again();

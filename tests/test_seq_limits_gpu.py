@@ -165,3 +165,22 @@ def test_hidden_keys_and_rows_in_use_at_every_width(D, aligned, causal, dtype):
         for n, t in got.items():
             ref.check(t, want[n], f"{n} hint {hint}")
     H.check_errors()
+
+
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_bias_gradient_of_fp32_has_no_drift_over_many_rows(D):
+    """The score gradients of a causal row cancel, so the bias gradient's sum over all buckets is zero, and what is left of it is the sum of
+    the rows' rounding errors.  Each is the error of do . v, weighted by p, and of do . o: both at most 6 D / 16 accumulator steps of 2^-24 of
+    sum |do||v|, uniform in that half step (2^-24 / sqrt 3).  Without a common sign T rows add up to sqrt(T) of it; 4 of these standard
+    deviations are allowed.  A rounding of one sign adds up to T of it."""
+    from scenario_wise_rec import ops
+    n, L, H = (16384, 50, 2) if D < 128 else (4096, 100, 2)
+    T = n * L
+    q, k, v, dout = (randn(10 + i, T, H, D) for i in range(4))
+    bias, table = randn(15, H, 8).mul_(0.5), ops.seq_buckets(8, 40)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, bias)]
+    out = ops.seq_attention(*leaves[:3], torch.arange(0, T + 1, L, dtype=torch.int32, device="cuda"), max_q=L, bias=bias, buckets=table)
+    drift = torch.autograd.grad(out, leaves, dout)[3].double().sum(1)
+    size = D * float(dout.abs().mean()) * float(v.detach().abs().mean())
+    row = 2 * (6 * D / 16) ** 0.5 * 2.0 ** -24 / 3 ** 0.5 * size
+    assert (drift.abs() <= 4 * T ** 0.5 * row).all(), (drift.tolist(), 4 * T ** 0.5 * row)
