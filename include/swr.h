@@ -818,6 +818,7 @@ int swr_block_select_bwd(const float* dout, int64_t ldo, const void* domain, int
  * q, k, v, dout: element strides row / head, unit stride inside a head; out, dq, dk, dv: contiguous [rows, heads, D], 16-byte aligned.
  * dtype SWR_F32 (products of three bf16 terms per value, fp32 accuracy) or SWR_BF16; bias, dbias, lse are fp32.
  * max_q / max_k: longest sequence -- they choose the launch and its tiling (right for any value, other values round differently).
+ * B * Hq up to 2^24 - 4096 fits a launch (fewer than 2^32 threads) whatever the lengths; what does not is SWR_ERR_UNSUPPORTED.
  * Deterministic: fixed summation orders, no atomics on results. */
 #define SWR_SEQ_MAX_DIM 128
 #define SWR_SEQ_MAX_DIST 2049

@@ -133,3 +133,14 @@ def test_norm_backward_refuses_a_missing_row_statistic():
     assert H.lib.swr_norm_gate_bwd(C.byref(a), None, 0, None) == -1
     a.rz = 4096                                            # (the next check is the workspace's)
     assert H.lib.swr_norm_gate_bwd(C.byref(a), None, 0, None) == -6
+
+
+def test_as_many_sequences_as_documented_fit():
+    """B * Hq = 2^24 - 4096 in any split over heads: a workspace (of the backward) is given, nothing is refused."""
+    from test_seq_ops_cpu import attention_args
+    import ctypes as C
+    from scenario_wise_rec import _hip as H
+    for Hq, Hk in ((1, 1), (4, 1), (4, 4), (64, 8), (32, 1)):
+        for D in (16, 33, 128):
+            a = attention_args(B=((1 << 24) - 4096) // Hq, Hq=Hq, Hk=Hk, D=D, max_q=5000, max_k=5000, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096)
+            assert H.lib.swr_seq_attention_bwd(C.byref(a), None, 0, None) == -6, (Hq, Hk, D)         # (only the workspace is missing)
